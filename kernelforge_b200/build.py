@@ -96,6 +96,20 @@ def ext_up_to_date() -> bool:
     return all(os.path.getmtime(f) <= t for f in deps)
 
 
+def _runtime_cxx_flags() -> list:
+    """Link against the libstdc++ this process has loaded (torch's), never a static copy.
+
+    A compiler installed without its shared libstdc++ links the archive instead, and two C++ runtimes
+    in one process do not share their locale: formatting a number in an error message then crashes.
+    """
+    with open("/proc/self/maps") as f:
+        for line in f:
+            path = line.rstrip("\n").split(None, 5)[-1]
+            if os.path.basename(path).startswith("libstdc++.so"):
+                return ["-nostdlib++", path]
+    return []
+
+
 def build_ext(force: bool = False, verbose: bool = False) -> str:
     """The torch extension (``kf_torch_ext.cpp``), linked against ``libkf_moe.so``."""
     if not force and ext_up_to_date():
@@ -108,7 +122,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     bdir = os.path.join(PKG, "_build", "torch_ext")
     os.makedirs(bdir, exist_ok=True)
     cpp_extension.load(name="_kf_torch", sources=[os.path.join(CSRC, EXT_SOURCE)], extra_include_paths=[INCLUDE],
-                       extra_cflags=["-O3"], extra_ldflags=[f"-L{PKG}", "-lkf_moe"], build_directory=bdir,
+                       extra_cflags=["-O3"], extra_ldflags=[f"-L{PKG}", "-lkf_moe", *_runtime_cxx_flags()], build_directory=bdir,
                        with_cuda=True, verbose=verbose)
     tmp = EXT + ".tmp"
     shutil.copyfile(os.path.join(bdir, "_kf_torch.so"), tmp)

@@ -182,3 +182,16 @@ def test_extension_loads_first_in_a_fresh_process():
             "ext = B.extension(); print(callable(ext.kernel))" % ROOT)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip().endswith("True"), r.stderr[-2000:]
+
+
+def test_torch_extension_shares_the_process_cxx_runtime():
+    """The extension needs the shared libstdc++ and carries no copy of its own (a second C++ runtime in
+    the process crashes as soon as an error message formats a number)."""
+    import subprocess
+    from kernelforge_b200 import build
+    B.extension()
+    needed = subprocess.run(["readelf", "-d", build.EXT], capture_output=True, text=True, check=True).stdout
+    assert "[libstdc++.so.6]" in needed
+    own = subprocess.run(["nm", "-D", "--defined-only", build.EXT], capture_output=True, text=True, check=True).stdout
+    # std::ostream::_M_insert<long>, std::locale::facet's vtable
+    assert not re.search(r" T _ZNSo9_M_insertIlEERSoT_\b| [VD] _ZTVNSt6locale5facetE\b", own)
