@@ -239,6 +239,99 @@ int kf_ep_combine(const void* partials, int32_t partials_fp32, const int32_t* po
 int kf_quantize_hidden(const void* x, int32_t num_tokens, void* out, float* out_scale, void* stream);
 
 /*
+ * ------------------------------------------------------------- training --
+ * Operators around a user's own expert products (the reference has none of
+ * them: its sort, SwiGLU and combine live inside kernel() without gradients).
+ * Rows are bf16, fp16 or fp32 (`dtype`), of any width; 16-byte aligned rows whose
+ * width is a multiple of 8 take 16-byte accesses, others one element at a time.
+ * A *_stride is the number of elements between an input's consecutive rows;
+ * outputs are dense.  Sums are fp32, in a fixed order, rounded once.
+ */
+#define KF_DTYPE_BF16 0
+#define KF_DTYPE_F16 1
+#define KF_DTYPE_F32 2
+
+#define KF_SORT_MAX_TOP_K 16
+#define KF_SORT_MAX_ALIGN 1024
+#define KF_SORT_MAX_WIDTH (1 << 20)
+#define KF_SORT_MAX_ROWS (1 << 30)
+
+/*
+ * Gradient of kf_moe_route's weights: grad_weight f32 [T, 8] -> grad_logits f32
+ * [T, 256], written in full (zero for experts not chosen).  The choice has no
+ * gradient and the bias takes part in the choice only.  Ids outside [0, 256)
+ * count as no choice.
+ */
+int kf_moe_route_backward(const float* routing_logits, const int32_t* topk_idx, const float* grad_weight,
+                          int32_t num_tokens, float routed_scaling_factor, float* grad_logits, void* stream);
+
+/*
+ * Tokens' rows in expert order.  topk_idx int32 [T, K] (1 <= K <= 16) holds global
+ * expert ids; the local experts are [expert_offset, expert_offset + num_experts),
+ * and every other id is a pair without a row.  Each (token, choice) pair of a
+ * local expert gets one row; an expert's rows are one segment, in (token, choice)
+ * order, that starts at a multiple of row_align.
+ *   rows      [num_rows, width]  rows[r] = x[token of row r], zeros where r has no pair
+ *   pair_row  int32 [T, K]       row of each pair, -1 without one
+ *   row_pair  int32 [num_rows]   pair t * K + k of each row, -1 without one
+ *   counts    int32 [E]          pairs of each expert
+ *   starts    int32 [E + 1]      segment starts, not beyond num_rows; starts[E] = their end
+ * num_rows is a multiple of row_align.  A pair whose row would lie at or past
+ * num_rows is dropped (its pair_row is -1; counts still counts it): pass at least
+ * T * K + min(T * K, E) * (row_align - 1) to keep all.  `workspace`:
+ * kf_sort_workspace_bytes(T, K, E) bytes.  Ids repeated in a token's choices are
+ * separate pairs.
+ */
+size_t kf_sort_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t num_experts);
+int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t* topk_idx, int32_t num_tokens,
+                   int32_t top_k, int32_t width, int32_t num_experts, int32_t expert_offset, int32_t row_align,
+                   int32_t num_rows, void* rows, int32_t* pair_row, int32_t* row_pair, int32_t* counts,
+                   int32_t* starts, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * output[t] = sum over k ascending of topk_weight[t, k] * rows[pair_row[t, k]] over
+ * the pairs that have a row (topk_weight f32 [T, K]; NULL: 1, which is the gradient
+ * of kf_sort_tokens with respect to x).  Rows without a pair are not read.
+ */
+int kf_combine_tokens(const void* rows, int32_t dtype, int64_t rows_stride, int32_t num_rows, const int32_t* pair_row,
+                      const float* topk_weight, int32_t num_tokens, int32_t top_k, int32_t width, void* output,
+                      void* stream);
+
+/*
+ * Gradients of kf_combine_tokens: grad_rows[r] = topk_weight[p] * grad_output[token]
+ * (zeros for a row without a pair), grad_weight[t, k] = <grad_output[t],
+ * rows[pair_row[t, k]]> (0 without a row).  Either output may be NULL.
+ */
+int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype, int64_t rows_stride, int32_t num_rows,
+                        const int32_t* pair_row, const int32_t* row_pair, const float* topk_weight, int32_t num_tokens,
+                        int32_t top_k, int32_t width, void* grad_rows, float* grad_weight, void* stream);
+
+/*
+ * Rows in 8 bits.  codes: e4m3 [R, W]; exponents: uint8 [R, ceil(W / 128)], value
+ * = code * 2^(exponent - 127) with one exponent per row and 128 columns, the
+ * smallest (>= 1) that holds the block's finite values within 448.  Values that
+ * are not finite are kept as NaN.  Codes end at 240 where 256 * 2^e is beyond the
+ * type.  kf_restore8 writes the values back: row i of output is row i, or, with
+ * row_pair (int32 [out_rows], from kf_sort_tokens), the row of token
+ * row_pair[i] / top_k, zeros where row_pair[i] is no pair.
+ */
+int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, int32_t width, void* codes,
+             void* exponents, void* stream);
+int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t num_rows, int32_t width,
+                const int32_t* row_pair, int32_t top_k, int32_t out_rows, void* output, void* stream);
+
+/*
+ * SwiGLU in the layer's column order, h [R, 2 I] = [up | gate], act = up * silu(gate)
+ * [R, I], with h kept in 8 bits: codes [R, 2 I], exponents [R, 2 ceil(I / 128)], the
+ * blocks of each half beginning at its own first column.  The backward pass reads
+ * what was kept: grad_h [R, 2 I], and act as the kept values give it (act may be NULL).
+ */
+int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_rows, int32_t inter, void* act,
+                    void* codes, void* exponents, void* stream);
+int kf_swiglu_backward8(const void* codes, const void* exponents, const void* grad_act, int32_t dtype,
+                        int64_t grad_stride, int32_t num_rows, int32_t inter, void* grad_h, void* act, void* stream);
+
+/*
  * Synchronises `stream`, then copies the device status word of the last call
  * that used `workspace` into *status (host pointer) and clears it.  Returns
  * KF_ERR_DEVICE_STATUS if any bit was set.

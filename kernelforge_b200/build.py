@@ -21,10 +21,10 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libkf_moe.so")
 EXT = os.path.join(PKG, "_kf_torch.so")
-EXT_SOURCE = "kf_torch_ext.cpp"
+EXT_SOURCES = ["kf_torch_ext.cpp", "kf_torch_train.cpp"]
 SOURCES = ["kf_route_permute.cu", "kf_grouped_gemm.cu", "kf_moe_api.cu",
-           "kf_moe_noalloc.cu", "kf_ep.cu", "kf_quant.cu"]
-HEADERS = ["kf_ptx.cuh", "kf_internal.cuh", "kf_quant.cuh", "kf_fp8.cuh"]
+           "kf_moe_noalloc.cu", "kf_ep.cu", "kf_quant.cu", "kf_sort.cu", "kf_rows8.cu", "kf_route_grad.cu"]
+HEADERS = ["kf_ptx.cuh", "kf_internal.cuh", "kf_quant.cuh", "kf_fp8.cuh", "kf_elem.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v", f"-I{INCLUDE}"]
@@ -92,7 +92,7 @@ def ext_up_to_date() -> bool:
     if not os.path.exists(EXT):
         return False
     t = os.path.getmtime(EXT)
-    deps = [os.path.join(CSRC, EXT_SOURCE), os.path.join(INCLUDE, "kf_moe.h"), LIB]
+    deps = [*(os.path.join(CSRC, f) for f in EXT_SOURCES), os.path.join(INCLUDE, "kf_moe.h"), LIB]
     return all(os.path.getmtime(f) <= t for f in deps)
 
 
@@ -111,7 +111,7 @@ def _runtime_cxx_flags() -> list:
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> str:
-    """The torch extension (``kf_torch_ext.cpp``), linked against ``libkf_moe.so``."""
+    """The torch extension (``kf_torch_ext.cpp``, ``kf_torch_train.cpp``), linked against ``libkf_moe.so``."""
     if not force and ext_up_to_date():
         return EXT
     import ctypes
@@ -121,7 +121,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     ctypes.CDLL(LIB)                      # its soname satisfies the extension's dependency when imported here
     bdir = os.path.join(PKG, "_build", "torch_ext")
     os.makedirs(bdir, exist_ok=True)
-    cpp_extension.load(name="_kf_torch", sources=[os.path.join(CSRC, EXT_SOURCE)], extra_include_paths=[INCLUDE],
+    cpp_extension.load(name="_kf_torch", sources=[os.path.join(CSRC, f) for f in EXT_SOURCES], extra_include_paths=[INCLUDE],
                        extra_cflags=["-O3"], extra_ldflags=[f"-L{PKG}", "-lkf_moe", *_runtime_cxx_flags()], build_directory=bdir,
                        with_cuda=True, verbose=verbose)
     tmp = EXT + ".tmp"

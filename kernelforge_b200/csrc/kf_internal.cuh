@@ -100,6 +100,9 @@ inline RowLayout packed_layout(const void* rows) {
                    kPackedRowBytes, reinterpret_cast<const float*>(b + kH), kPackedRowBytes / 4, 1};
 }
 
+// KF_OK on a B200, with its SM count (sets the current device up on first use).
+int device_ready(int* num_sms);
+
 // Every kernel of the layer's launch chain is launched with programmatic stream
 // serialization: it may start while its predecessor in the stream is finishing,
 // and begins with grid_dep_wait().

@@ -287,6 +287,8 @@ int run_front_small(const Workspace& w, void* ws, const float* logits, const voi
 
 }  // namespace
 
+int device_ready(int* num_sms) { return ensure_device(num_sms); }
+
 Workspace plan_workspace(int32_t T, int32_t E) {
   Workspace w{};
   const int64_t pairs_max = static_cast<int64_t>(T) * (E < kTopK ? E : kTopK);

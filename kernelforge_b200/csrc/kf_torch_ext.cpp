@@ -29,6 +29,8 @@
 
 #include "kf_moe.h"
 
+void register_train(pybind11::module_& m);  // kf_torch_train.cpp
+
 namespace {
 
 constexpr int64_t kH = KF_MOE_HIDDEN, kI = KF_MOE_INTERMEDIATE, kEG = KF_MOE_GLOBAL_EXPERTS, kB = KF_MOE_BLOCK;
@@ -169,4 +171,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kernel", &kernel, "the fused MoE layer (kf_moe_forward); returns bf16 [T, 7168]");
   m.def("read_status", &read_status, "synchronise and return, then clear, the device status of this module's calls");
   m.def("release_workspaces", &release_workspaces, "drop the cached workspaces");
+  register_train(m);
 }

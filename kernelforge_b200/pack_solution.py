@@ -43,7 +43,7 @@ def source_files() -> List[str]:
     """Repository-relative paths of every file the packed solution carries."""
     from . import build
     files = [os.path.join("kernelforge_b200", f) for f in PY_SOURCES]
-    files += [os.path.join("kernelforge_b200", "csrc", f) for f in build.SOURCES + build.HEADERS + [build.EXT_SOURCE]]
+    files += [os.path.join("kernelforge_b200", "csrc", f) for f in build.SOURCES + build.HEADERS + build.EXT_SOURCES]
     files.append(os.path.join("include", "kf_moe.h"))
     return files
 

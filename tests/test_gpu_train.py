@@ -1,0 +1,520 @@
+"""The training operators on a B200 against their definitions in 64 bits (``train_reference``).
+
+Tolerances.  A result is one fp32 computation rounded once to its type: half a step of the type
+(``R.half_step``) on top of the fp32 operations' own 2^-24 each.  A sum of n terms is off by at
+most n * 2^-24 times the sum of their magnitudes; a dot product over the width passes every term
+through at most 8 additions per 256 columns of one warp, 5 in the warp and 16 across warps.  A
+sigmoid from expf (2 ulp), an addition and a division is within 2^-21, and the products around
+it add a few 2^-24: 2^-20 of the magnitudes in all.  Where e^-g leaves fp32's normal numbers
+(g below -87.3, 1 + e^-g above 2^126) the sigmoid, at most 2^-126, may come out as zero: FAR of
+the magnitudes around it.
+"""
+import pytest
+import torch
+
+from kernelforge_b200 import binding as B
+from kernelforge_b200 import train
+from tests import train_reference as R
+from tests.helpers import gpu_available
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a B200")]
+
+U = 2.0 ** -24
+FAR = 2.0 ** -126
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _ids(t, k, g, masked=0.0, experts=256):
+    """Distinct experts per token, some more popular than others; masked tokens have none."""
+    score = torch.randn(t, 256, generator=g) + torch.randn(256, generator=g)
+    ids = score.topk(k, dim=1).indices.to(torch.int32)
+    ids[torch.rand(t, generator=g) < masked] = -1
+    return ids
+
+
+def _dot_slack(h):
+    return (8 * ((h + 255) // 256) + 21) * U
+
+
+def _order(case, ids):
+    t, k = ids.shape
+    rows = case.get("max_rows") or R.worst_rows(t, k, case["experts"], case["align"])
+    return R.order(ids, case["experts"], case["offset"], case["align"], rows), rows
+
+
+def _same_order(order, ref):
+    for got, want in zip(order, ref):
+        assert got.dtype == torch.int32 and torch.equal(got.cpu(), want)
+
+
+SORT_CASES = [
+    # tokens, k, hidden, experts, offset, align, masked share, bound on the rows
+    dict(t=1, k=1, h=64, experts=256, offset=0, align=1, masked=0.0),
+    dict(t=1, k=8, h=7168, experts=256, offset=0, align=1, masked=0.0),
+    dict(t=5, k=16, h=1, experts=256, offset=0, align=1, masked=0.3),
+    dict(t=16, k=8, h=7168, experts=32, offset=96, align=128, masked=0.0),
+    dict(t=33, k=3, h=1031, experts=100, offset=156, align=8, masked=0.3),
+    dict(t=129, k=2, h=520, experts=1, offset=7, align=16, masked=0.0),
+    dict(t=300, k=8, h=264, experts=256, offset=0, align=1, masked=0.5),
+    dict(t=513, k=7, h=200, experts=64, offset=64, align=1024, masked=0.0),
+    dict(t=1000, k=8, h=96, experts=256, offset=0, align=16, masked=0.1, max_rows=4000),
+    dict(t=64, k=4, h=136, experts=256, offset=0, align=1, masked=0.0, max_rows=1),
+    dict(t=7000, k=8, h=24, experts=256, offset=0, align=8, masked=0.0),
+    dict(t=40, k=8, h=80, experts=256, offset=0, align=4, masked=1.0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", SORT_CASES, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_sort_and_its_gradient(case, dtype):
+    g = torch.Generator().manual_seed(case["t"] * 31 + case["k"])
+    t, k, h = case["t"], case["k"], case["h"]
+    ids = _ids(t, k, g, case["masked"])
+    ref, rows = _order(case, ids)
+    x = torch.randn(t, h, generator=g).to(dtype)
+    xg = x.cuda().requires_grad_(True)
+    out, order = train.sort_tokens(xg, ids.cuda(), case["experts"], case["offset"], row_align=case["align"],
+                                   max_rows=case.get("max_rows"))
+    _same_order(order, ref)
+    assert out.dtype == dtype and torch.equal(out.detach().cpu(), R.gather(x, ref[1], k))
+    grad = torch.randn(rows, h, generator=g).to(dtype)
+    grad[ref[1] < 0] = float("nan")          # rows of no pair must not be read
+    dx, = torch.autograd.grad(out, xg, grad.cuda())
+    want, mag = R.combine(grad, ref[0])
+    R.close(dx, want, dtype, k * U * mag)
+    assert torch.equal(train.sort_tokens_backward(grad.cuda(), order), dx)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", SORT_CASES, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_combine_and_its_gradients(case, dtype):
+    g = torch.Generator().manual_seed(case["t"] * 17 + case["k"])
+    t, k, h = case["t"], case["k"], case["h"]
+    ids = _ids(t, k, g, case["masked"])
+    ref, rows = _order(case, ids)
+    order = train.TokenOrder(*(a.cuda() for a in ref))
+    y = torch.randn(rows, h, generator=g).to(dtype)
+    y[ref[1] < 0] = float("inf")
+    w = torch.randn(t, k, generator=g)
+    w[ref[0] < 0] = float("nan")             # weights of pairs without a row are not used
+    dout = torch.randn(t, h, generator=g).to(dtype)
+    yg, wg = y.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    out = train.combine_tokens(yg, order, wg)
+    want, mag = R.combine(y, ref[0], w)
+    R.close(out.detach(), want, dtype, (k + 1) * U * mag)
+    dy, dw = torch.autograd.grad(out, (yg, wg), dout.cuda())
+    want_rows, want_w, mag_w = R.combine_grads(dout, y, ref[0], ref[1], w)
+    R.close(dy, want_rows, dtype, U * want_rows.abs())
+    R.close(dw, want_w, torch.float32, _dot_slack(h) * mag_w)
+    both = train.combine_tokens_backward(dout.cuda(), y.cuda(), order, w.cuda())
+    assert torch.equal(both[0], dy) and torch.equal(both[1], dw)
+    # one gradient alone, and no weights
+    yg2 = y.cuda().requires_grad_(True)
+    dy2, = torch.autograd.grad(train.combine_tokens(yg2, order, w.cuda()), yg2, dout.cuda())
+    assert torch.equal(dy2, dy)
+    wg2 = w.cuda().requires_grad_(True)
+    dw2, = torch.autograd.grad(train.combine_tokens(y.cuda(), order, wg2), wg2, dout.cuda())
+    assert torch.equal(dw2, dw)
+    plain, mag = R.combine(y, ref[0])
+    R.close(train.combine_tokens(y.cuda(), order), plain, dtype, k * U * mag)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h", [264, 131])
+def test_rows_in_place_of_other_layouts(h, dtype):
+    """Strided rows, rows off a 16-byte boundary, transposed rows, and expanded gradients."""
+    g = torch.Generator().manual_seed(h)
+    t, k = 50, 4
+    ids = _ids(t, k, g)
+    big = torch.randn(t, 2 * h + 3, generator=g).to(dtype).cuda()
+    case = dict(experts=256, offset=0, align=8)
+    ref, rows = _order(case, ids)
+    for x in (big[:, :h], big[:, 3:3 + h], big[:, 8:8 + h], torch.randn(h, t, generator=g).to(dtype).cuda().t(),
+              big[:1, :h].expand(t, h)):
+        out, order = train.sort_tokens(x, ids.cuda(), 256, row_align=8)
+        assert torch.equal(out.cpu(), R.gather(x.cpu(), ref[1], k))
+        kept = train.pack8(x)
+        same = train.pack8(x.contiguous())
+        assert torch.equal(kept.codes.view(torch.uint8), same.codes.view(torch.uint8)) and torch.equal(kept.exponents, same.exponents)
+    wide = torch.randn(rows, h + 5, generator=g).to(dtype).cuda()
+    order = train.TokenOrder(*(a.cuda() for a in ref))
+    w = torch.rand(t, k, generator=g)
+    want, mag = R.combine(wide[:, 2:2 + h].cpu(), ref[0], w)
+    y = wide[:, 2:2 + h].detach().requires_grad_(True)
+    out = train.combine_tokens(y, order, w.t().contiguous().t().cuda())
+    R.close(out.detach(), want, dtype, (k + 1) * U * mag)
+    dy, = torch.autograd.grad(out.sum(), y)      # an expanded gradient
+    R.close(dy, R.combine_grads(torch.ones(t, h), wide[:, 2:2 + h].cpu(), ref[0], ref[1], w)[0], dtype, 0.0)
+
+
+def test_sort_of_repeated_and_foreign_ids():
+    ids = torch.tensor([[3, 3, 3], [300, -5, 3], [2 ** 31 - 1, -2 ** 31, 255], [0, 255, 0]], dtype=torch.int32)
+    x = torch.randn(4, 16)
+    ref = R.order(ids, 256, 0, 2, R.worst_rows(4, 3, 256, 2))
+    out, order = train.sort_tokens(x.cuda(), ids.cuda(), 256, row_align=2)
+    _same_order(order, ref)
+    assert torch.equal(out.cpu(), R.gather(x, ref[1], 3))
+    shifted, order = train.sort_tokens(x.cuda(), ids.cuda(), 200, 56)
+    _same_order(order, R.order(ids, 200, 56, 1, 12))
+
+
+def test_sort_without_tokens_or_rows():
+    out, order = train.sort_tokens(torch.empty(0, 32).cuda(), torch.empty(0, 8, dtype=torch.int32).cuda(), 12)
+    assert out.shape == (0, 32) and order.pair_row.shape == (0, 8) and order.row_pair.shape == (0,)
+    assert not order.counts.any() and not order.starts.any()
+    out, order = train.sort_tokens(torch.empty(0, 32).cuda(), torch.empty(0, 8, dtype=torch.int32).cuda(), 12, row_align=4, max_rows=8)
+    assert not out.any() and (order.row_pair == -1).all() and out.shape == (8, 32)
+    x = torch.randn(3, 32).cuda()
+    ids = torch.zeros(3, 2, dtype=torch.int32).cuda()
+    out, order = train.sort_tokens(x, ids, 12, max_rows=0)
+    assert out.shape == (0, 32) and (order.pair_row == -1).all() and int(order.counts[0]) == 6
+    assert not train.combine_tokens(out, order, torch.ones(3, 2).cuda()).any()
+    assert train.combine_tokens(torch.empty(0, 32).cuda(), train.TokenOrder(
+        torch.empty(0, 2, dtype=torch.int32).cuda(), torch.empty(0, dtype=torch.int32).cuda(), order.counts, order.starts)).shape == (0, 32)
+    assert train.pack8(torch.empty(0, 32).cuda()).codes.shape == (0, 32)
+    assert train.swiglu(torch.empty(0, 32).cuda()).shape == (0, 16)
+
+
+def test_an_order_that_does_not_fit_is_harmless():
+    """Rows or pairs out of range in a caller's order count as none (no read or write out of range)."""
+    pair_row = torch.tensor([[0, 7], [2 ** 31 - 1, -9]], dtype=torch.int32).cuda()
+    row_pair = torch.tensor([0, 99, -7, 2 ** 31 - 1], dtype=torch.int32).cuda()
+    order = train.TokenOrder(pair_row, row_pair, pair_row[0], pair_row[0])
+    y = torch.randn(4, 40).cuda()
+    w = torch.ones(2, 2).cuda()
+    out = train.combine_tokens(y, order, w)
+    assert torch.equal(out[0], y[0]) and not out[1].any()
+    dr, dw = train.combine_tokens_backward(torch.ones(2, 40).cuda(), y, order, w)
+    assert (dr[0] == 1).all() and not dr[1:].any() and not dw[1].any() and dw[0, 1] == 0
+    back = train.restore8(train.pack8(y[:2].contiguous()), order)
+    assert not back[1:].any()
+
+
+# ---------------------------------------------------------------------- route --
+
+
+@pytest.mark.parametrize("t", [1, 7, 64, 1000])
+def test_route_and_its_gradient(t):
+    g = torch.Generator().manual_seed(t)
+    logits = torch.randn(t, 256, generator=g)
+    bias = (0.02 * torch.randn(256, generator=g)).to(torch.bfloat16)
+    lg = logits.cuda().requires_grad_(True)
+    idx, w = train.route(lg, bias.cuda(), 2.5)
+    idx0, w0 = B.route(logits.cuda(), bias.cuda(), 2.5)
+    assert torch.equal(idx, idx0) and torch.equal(w.detach(), w0)
+    gw = torch.randn(t, 8, generator=g)
+    dl, = torch.autograd.grad(w, lg, gw.cuda())
+    want, mag = R.route_grad(logits, idx.cpu(), gw, 2.5)
+    R.close(dl, want, torch.float32, 2.0 ** -19 * mag)
+    assert torch.equal(dl, train.route_backward(logits.cuda(), idx, gw.cuda(), 2.5))
+
+
+def test_route_gradient_at_the_ends():
+    """Saturated logits, ids of no choice and a token without any."""
+    g = torch.Generator().manual_seed(1)
+    logits = 30 * torch.randn(40, 256, generator=g)
+    ids = torch.stack([torch.randperm(256, generator=g)[:8] for _ in range(40)]).to(torch.int32)
+    ids[3] = -1
+    ids[4, ::2] = 256
+    gw = torch.randn(40, 8, generator=g)
+    gw[3] = float("nan")
+    dl = train.route_backward(logits.cuda(), ids.cuda(), gw.cuda(), 1.5)
+    want, mag = R.route_grad(logits, ids, torch.nan_to_num(gw), 1.5)
+    # sigmoids down to e^-100 lose their last bits as fp32 subnormals: what they weigh is below 1e-30
+    R.close(dl, want, torch.float32, 2.0 ** -19 * mag + 1e-30)
+    assert not dl[3].any()
+
+
+# --------------------------------------------------------------------- 8 bits --
+
+
+def _rows(r, w, dtype, g):
+    x = torch.randn(r, w, generator=g) * torch.exp(2 * torch.randn(r, 1, generator=g))
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("r,w", [(1, 1), (3, 127), (2, 128), (5, 136), (4, 1000), (17, 257), (64, 7168), (9, 2047)])
+def test_rows_in_8_bits_and_back(r, w, dtype):
+    g = torch.Generator().manual_seed(r + w)
+    x = _rows(r, w, dtype, g)
+    kept = train.pack8(x.cuda())
+    want, e = R.to_8_bits(x)
+    assert kept.dtype == dtype and torch.equal(kept.exponents.cpu().double() - 127, e)
+    back = train.restore8(kept)
+    assert back.dtype == dtype and torch.equal(back.cpu().double(), want.to(dtype).double())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("w", [256, 131])
+def test_rows_in_8_bits_at_the_ends(w, dtype):
+    """Zeros, the type's largest and smallest values, values next to a border, and values that are not finite."""
+    info = torch.finfo(dtype)
+    rows = [torch.zeros(w), torch.full((w,), info.max), torch.full((w,), -info.max), torch.full((w,), info.tiny),
+            torch.linspace(-1, 1, w) * info.max, torch.linspace(-448, 448, w), torch.linspace(-1, 1, w) * 449,
+            torch.linspace(-17.5, 17.5, w), 2.0 ** torch.linspace(-24, 15, w), torch.linspace(0, 2.0 ** -9, w)]
+    odd = torch.linspace(-3, 3, w)
+    odd[5], odd[7], odd[w - 1] = float("inf"), float("nan"), float("-inf")
+    rows += [odd, torch.full((w,), float("nan")), torch.full((w,), float("inf"))]
+    x = torch.stack(rows).to(dtype)
+    want, e = R.to_8_bits(x)
+    kept = train.pack8(x.cuda())
+    assert torch.equal(kept.exponents.cpu().double() - 127, e)
+    back = train.restore8(kept).cpu()
+    finite = torch.isfinite(x)
+    assert torch.isnan(back[~finite]).all() and torch.isfinite(back[finite]).all()
+    assert torch.equal(back[finite].double(), want.to(dtype)[finite].double())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", SORT_CASES[1:9], ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_rows_in_8_bits_in_expert_order(case, dtype):
+    g = torch.Generator().manual_seed(case["t"])
+    ids = _ids(case["t"], case["k"], g, case["masked"])
+    ref, _ = _order(case, ids)
+    x = _rows(case["t"], case["h"], dtype, g)
+    back = train.restore8(train.pack8(x.cuda()), train.TokenOrder(*(a.cuda() for a in ref)))
+    assert torch.equal(back.cpu(), R.gather(R.to_8_bits(x)[0].to(dtype), ref[1], case["k"]))
+
+
+# --------------------------------------------------------------------- swiglu --
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("r,n", [(1, 1), (1, 128), (3, 131), (7, 1368), (33, 2048), (130, 264)])
+def test_swiglu_and_its_gradient(r, n, dtype):
+    g = torch.Generator().manual_seed(r * n)
+    h = _rows(r, 2 * n, dtype, g)
+    d = torch.randn(r, n, generator=g).to(dtype)
+    act, kept = train.swiglu_pack8(h.cuda())
+    u, gate = h[:, :n].double(), h[:, n:].double()
+    R.close(act, R.swiglu(u, gate), dtype, 2.0 ** -20 * R.swiglu(u, gate).abs() + FAR * (u * gate).abs())
+    (ku, eu), (kg, eg) = R.to_8_bits(h[:, :n]), R.to_8_bits(h[:, n:])
+    assert torch.equal(kept.exponents.cpu().double() - 127, torch.cat([eu, eg], 1))
+    dh, again = train.swiglu_backward8(kept, d.cuda())
+    du, dg, a, mag = R.swiglu_grads(ku, kg, d.double())
+    dd = d.double()
+    R.close(again, a, dtype, 2.0 ** -20 * a.abs() + FAR * (ku * kg).abs())
+    R.close(dh[:, :n], du, dtype, 2.0 ** -20 * du.abs() + FAR * (dd * kg).abs())
+    R.close(dh[:, n:], dg, dtype, 2.0 ** -20 * mag + FAR * (dd * ku).abs() * (1 + kg.abs()))
+    hg = h.cuda().requires_grad_(True)
+    out = train.swiglu(hg)
+    dh2, = torch.autograd.grad(out, hg, d.cuda())
+    assert torch.equal(out.detach(), act) and torch.equal(dh2, dh)
+    assert torch.equal(train.swiglu(h.cuda()), act)
+    only, none = train.swiglu_backward8(kept, d.cuda(), need_act=False)
+    assert none is None and torch.equal(only, dh)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_swiglu_of_far_gates(dtype):
+    gate = torch.tensor([-60000.0, -1000, -90, -88, -40, -20, -1e-6, 0, 1e-6, 20, 90, 1000, 60000]).to(dtype)
+    h = torch.cat([torch.ones_like(gate), gate])[None]
+    n = gate.numel()
+    act, kept = train.swiglu_pack8(h.cuda())
+    # a sigmoid below fp32's smallest normal value may come out as zero: |gate| * 2^-126
+    R.close(act, R.swiglu(h[:, :n].double(), h[:, n:].double()), dtype, 2.0 ** -18 * R.swiglu(h[:, :n].double(), h[:, n:].double()).abs() + 1e-33)
+    dh, again = train.swiglu_backward8(kept, torch.ones(1, n).to(dtype).cuda())
+    assert torch.isfinite(dh).all() and torch.isfinite(again).all()
+
+
+# ------------------------------------------------------------------- together --
+
+
+def test_refusals_on_the_gpu():
+    x, ids = torch.zeros(4, 32).cuda(), torch.zeros(4, 2, dtype=torch.int32).cuda()
+    _, order = train.sort_tokens(x, ids, 8)
+    w = torch.ones(4, 2).cuda()
+    kept = train.pack8(x)
+    bad = [lambda: train.sort_tokens(x.double(), ids, 8), lambda: train.sort_tokens(x[0], ids, 8),
+           lambda: train.sort_tokens(x, ids.long(), 8), lambda: train.sort_tokens(x, ids[:3], 8),
+           lambda: train.sort_tokens(x, ids.cpu(), 8), lambda: train.sort_tokens(x, ids, 0),
+           lambda: train.sort_tokens(x, ids, 257), lambda: train.sort_tokens(x, ids, 8, 250),
+           lambda: train.sort_tokens(x, ids, 8, -1), lambda: train.sort_tokens(x, ids, 8, row_align=0),
+           lambda: train.sort_tokens(x, ids, 8, row_align=2000), lambda: train.sort_tokens(x, ids, 8, row_align=8, max_rows=12),
+           lambda: train.sort_tokens(x, ids, 8, max_rows=-1), lambda: train.sort_tokens(x, ids, 8, max_rows=2 ** 31),
+           lambda: train.sort_tokens(x[:, :0], ids, 8), lambda: train.sort_tokens(x, ids.expand(4, 2).repeat(1, 9), 8),
+           lambda: train.combine_tokens(x, order, w), lambda: train.combine_tokens(torch.zeros(8, 32).cuda(), order, w.double()),
+           lambda: train.combine_tokens(torch.zeros(8, 32).cuda(), order, w[:, :1]),
+           lambda: train.combine_tokens(torch.zeros(8, 32).cuda().long(), order, w),
+           lambda: train.sort_tokens_backward(x, order),
+           lambda: train.combine_tokens_backward(x, torch.zeros(8, 16).cuda(), order, w),
+           lambda: train.combine_tokens_backward(x[:3], torch.zeros(8, 32).cuda(), order, w),
+           lambda: train.restore8(kept._replace(exponents=kept.exponents[:3])), lambda: train.restore8(kept._replace(dtype=torch.int32)),
+           lambda: train.restore8(train.pack8(x[:3]), order), lambda: train.swiglu(x[:, :31]),
+           lambda: train.swiglu_backward8(kept, x), lambda: train.swiglu_backward8(train.swiglu_pack8(x)[1], x),
+           lambda: train.route_backward(torch.zeros(4, 256).cuda(), ids, w, 1.0),
+           lambda: train.route(torch.zeros(4, 255).cuda(), torch.zeros(255, dtype=torch.bfloat16).cuda(), 1.0)]
+    for i, call in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+            pytest.fail(f"call {i} was accepted")
+
+
+def test_no_second_derivative():
+    x = torch.randn(4, 32).cuda().requires_grad_(True)
+    rows, order = train.sort_tokens(x, torch.zeros(4, 2, dtype=torch.int32).cuda(), 8)
+    for out in (rows, train.swiglu(x), train.combine_tokens(rows, order)):
+        with pytest.raises(RuntimeError, match="not twice differentiable"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+def _layer(x, logits, bias, w13, w2, products):
+    """An MoE layer with the caller's own expert products."""
+    idx, weight = train.route(logits, bias, 2.5)
+    rows, order = train.sort_tokens(x, idx, w13.shape[0], row_align=8)
+    h = products(rows, order, w13)
+    y = products(train.swiglu(h), order, w2)
+    return train.combine_tokens(y, order, weight), order, idx
+
+
+def _products(rows, order, w):
+    """Each expert's rows times its matrix, a segment at a time (fp32)."""
+    starts = order.starts.tolist()
+    parts = [rows[starts[e]:starts[e + 1]] @ w[e].t() for e in range(w.shape[0])]
+    return torch.cat(parts + [rows.new_zeros(rows.shape[0] - starts[-1], w.shape[1])])
+
+
+def test_the_operators_together_as_a_layer():
+    """A whole fp32 layer, forward and every gradient, against the same layer in 64 bits.
+
+    The 64-bit layer's backward pass takes SwiGLU's input as the 8-bit form keeps it, as the operator
+    documents.  fp32 products over 48 and 32 columns and the operators' own sums: 200 roundings of 2^-24 of
+    the largest magnitudes at most, against outputs and gradients compared at their largest value; 1e-4 of
+    it is that with a factor of 8 for cancellation inside the sums.  A kept value may fall on the other side of an
+    e4m3 border than the 64-bit one (h differs by fp32 rounding): the 64-bit layer keeps the fp32 h's values.
+    """
+    g = torch.Generator().manual_seed(11)
+    t, h, n, experts = 70, 48, 32, 256
+    x = torch.randn(t, h, generator=g)
+    logits = torch.randn(t, 256, generator=g)
+    bias = (0.02 * torch.randn(256, generator=g)).to(torch.bfloat16)
+    w13 = 0.2 * torch.randn(experts, 2 * n, h, generator=g)
+    w2 = 0.2 * torch.randn(experts, h, n, generator=g)
+    dout = torch.randn(t, h, generator=g)
+    leaves = [a.cuda().requires_grad_(True) for a in (x, logits, w13, w2)]
+    kept = {}
+
+    def products(rows, order, w):
+        out = _products(rows, order, w)
+        kept.setdefault("h", out.detach().cpu())
+        return out
+
+    torch.backends.cuda.matmul.allow_tf32 = False
+    out, order, idx = _layer(leaves[0], leaves[1], bias.cuda(), leaves[2], leaves[3], products)
+    grads = torch.autograd.grad(out, leaves, dout.cuda())
+
+    xd, ld, w13d, w2d = (a.double().requires_grad_(True) for a in (x, logits, w13, w2))
+    idx, pair_row, row_pair = idx.cpu(), order.pair_row.cpu(), order.row_pair.cpu()
+    s = torch.sigmoid(ld.gather(1, idx.long()))
+    weight = 2.5 * s / (s.sum(1, keepdim=True) + 1e-20)
+    q = torch.cat([R.to_8_bits(kept["h"][:, :n])[0], R.to_8_bits(kept["h"][:, n:])[0]], 1)
+    want = torch.zeros(t, h, dtype=torch.float64)
+    for tok in range(t):
+        for k in range(8):
+            e = int(idx[tok, k])
+            hh = w13d[e] @ xd[tok]
+            exact_act = R.swiglu(hh[:n], hh[n:])
+            kq = q[int(pair_row[tok, k])] + (hh - hh.detach())        # the kept value, with h's gradient
+            act = R.swiglu(kq[:n], kq[n:])
+            act = exact_act.detach() + (act - act.detach())           # the forward value, the kept value's gradient
+            want[tok] = want[tok] + weight[tok, k] * (w2d[e] @ act)
+    wants = torch.autograd.grad(want, (xd, ld, w13d, w2d), dout.double())
+    for got, ref in zip((out.detach(),) + grads, (want.detach(),) + wants):
+        assert (got.double().cpu() - ref).abs().max() <= 1e-4 * ref.abs().max()
+
+
+def _training_calls(x, ids, w, dout, d8):
+    rows, order = train.sort_tokens(x, ids, 256, row_align=8)
+    out = train.combine_tokens(rows, order, w)
+    drows, dw = train.combine_tokens_backward(dout, rows, order, w)
+    dx = train.sort_tokens_backward(drows, order)
+    act, kept = train.swiglu_pack8(rows)
+    dh, again = train.swiglu_backward8(kept, d8)
+    back = train.restore8(train.pack8(x), order)
+    return (rows, *order, out, drows, dw, dx, act, dh, again, back)
+
+
+def _inputs(seed, t=200, h=320, k=8):
+    g = torch.Generator().manual_seed(seed)
+    rows = R.worst_rows(t, k, 256, 8)
+    return [a.cuda() for a in (torch.randn(t, h, generator=g).to(torch.bfloat16), _ids(t, k, g, 0.1),
+                               torch.rand(t, k, generator=g), torch.randn(t, h, generator=g).to(torch.bfloat16),
+                               torch.randn(rows, h // 2, generator=g).to(torch.bfloat16))]
+
+
+@pytest.mark.parametrize("t", [3, 200, 6000])
+def test_captured_and_replayed(t):
+    """Two graphs captured one after the other and replayed in turn on new inputs give the direct calls' bits."""
+    a, b = _inputs(1, t), _inputs(2, t)
+    want = [[o.clone() for o in _training_calls(*i)] for i in (a, b)]
+    torch.cuda.synchronize()
+    graphs, static, outs = [], [], []
+    for i in (a, b):
+        static.append([torch.zeros_like(v) for v in i])
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(_training_calls(*static[-1]))
+        graphs.append(gr)
+    for _ in range(2):
+        for i, gr, s in ((a, graphs[0], static[0]), (b, graphs[1], static[1])):
+            for dst, src in zip(s, i):
+                dst.copy_(src)
+            gr.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x.nan_to_num(), y.nan_to_num()) for x, y in zip(o, w))
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams share nothing."""
+    inputs = [_inputs(3, 6000), _inputs(4, 6000)]
+    want = [[o.clone() for o in _training_calls(*i)] for i in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    got = [None, None]
+    for _ in range(3):
+        for n, (s, i) in enumerate(zip(streams, inputs)):
+            with torch.cuda.stream(s):
+                got[n] = _training_calls(*i)
+    torch.cuda.synchronize()
+    for o, w in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(o, w))
+
+
+def test_equal_inputs_give_equal_bits():
+    i = _inputs(5, 3000)
+    first = [o.clone() for o in _training_calls(*i)]
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(first, _training_calls(*i)))
+
+
+@pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_on_a_device_that_is_not_current():
+    i = _inputs(6)
+    want = _training_calls(*i)
+    got = _training_calls(*(v.to("cuda:1") for v in i))
+    assert all(o.device.index == 1 and torch.equal(o.cpu(), w.cpu()) for o, w in zip(got, want))
+
+
+def test_rows_past_32_bit_offsets():
+    """A buffer of more than 2^31 elements: the last segment's rows lie past 32-bit offsets."""
+    t, h, k = 40960, 7168, 8          # 327680 rows of 7168: 2.35e9 elements
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(t, h, generator=g, device="cuda").to(torch.bfloat16)
+    ids = torch.randn(t, 256, generator=g, device="cuda").topk(k, dim=1).indices.to(torch.int32)
+    rows, order = train.sort_tokens(x, ids, 256)
+    assert rows.numel() > 2 ** 31
+    pick = torch.cat([torch.arange(3), torch.randint(0, rows.shape[0], (2000,), device="cuda", generator=g).cpu(),
+                      torch.arange(rows.shape[0] - 3, rows.shape[0])]).cuda()
+    pair = order.row_pair[pick].long()
+    assert torch.equal(rows[pick], x[pair // k])
+    assert torch.equal(order.pair_row.reshape(-1)[pair].long(), pick)
+    w = torch.full((t, k), 0.125, device="cuda")
+    assert torch.equal(train.combine_tokens(rows, order, w), x)       # eight equal rows times 1/8: exact
+    drows, dw = train.combine_tokens_backward(x, rows, order, w)
+    assert torch.equal(drows[pick], (x[pair // k].float() * 0.125).to(torch.bfloat16))
+    want = (x[:64].double() ** 2).sum(1, keepdim=True)
+    assert ((dw[:64].double() - want).abs() <= _dot_slack(h) * want).all()
+    back = train.restore8(train.pack8(x), order)
+    assert torch.equal(back[pick], train.restore8(train.pack8(x))[pair // k])
