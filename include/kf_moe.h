@@ -312,18 +312,20 @@ int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype
  * smallest (>= 1) that holds the block's finite values within 448.  Values that
  * are not finite are kept as NaN.  Codes end at 240 where 256 * 2^e is beyond the
  * type.  kf_restore8 writes the values back: row i of output is row i, or, with
- * row_pair (int32 [out_rows], from kf_sort_tokens), the row of token
- * row_pair[i] / top_k, zeros where row_pair[i] is no pair.
+ * pair_row (int32 [num_rows, top_k]) and row_pair (int32 [out_rows]) of
+ * kf_sort_tokens, token t's row goes to the rows pair_row[t, :], and the rows
+ * that row_pair gives no pair are zero.
  */
 int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, int32_t width, void* codes,
              void* exponents, void* stream);
 int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t num_rows, int32_t width,
-                const int32_t* row_pair, int32_t top_k, int32_t out_rows, void* output, void* stream);
+                const int32_t* pair_row, const int32_t* row_pair, int32_t top_k, int32_t out_rows, void* output,
+                void* stream);
 
 /*
  * SwiGLU in the layer's column order, h [R, 2 I] = [up | gate], act = up * silu(gate)
  * [R, I], with h kept in 8 bits: codes [R, 2 I], exponents [R, 2 ceil(I / 128)], the
- * blocks of each half beginning at its own first column.  The backward pass reads
+ * blocks of each half beginning at its own first column (both NULL: act alone).  The backward pass reads
  * what was kept: grad_h [R, 2 I], and act as the kept values give it (act may be NULL).
  */
 int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_rows, int32_t inter, void* act,

@@ -1,9 +1,10 @@
 // Rows of bf16, fp16 or fp32 elements, read and written eight columns per lane.
 //
-// A warp covers a slice of 256 columns.  In the vector form (kVec) lane l holds
-// columns 8l .. 8l+7 in 16-byte accesses, which needs 16-byte aligned rows and a
-// width that is a multiple of 8; otherwise lane l holds columns l + 32 j, one
-// element per access, so that a warp's accesses still fall in whole sectors.
+// A warp covers a slice of 256 columns.  In the vector form (kVec), which needs
+// 16-byte aligned rows and a width that is a multiple of 8, a lane's accesses are 16
+// bytes: lane l holds columns 8l .. 8l+7 of 16-bit types, and 4l .. 4l+3 and
+// 128 + 4l .. 128 + 4l+3 of fp32, so that each access of a warp is one run of 512
+// bytes.  Otherwise lane l holds columns l + 32 j, one element per access.
 // Arithmetic is fp32 whatever the element type.
 #pragma once
 
@@ -54,10 +55,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Column of element j of this lane inside a slice.
-template <bool kVec>
-__device__ __forceinline__ int slice_col(int lane, int j) {
-  return kVec ? lane * 8 + j : lane + 32 * j;
+// Column of a lane's 16-byte access i (of 1 for 16-bit types, 2 for fp32) inside a slice.
+template <typename T>
+__device__ __forceinline__ int vec_col(int lane, int i) {
+  return i * 128 + lane * (16 / static_cast<int>(sizeof(T)));
 }
 
 // The raw bits of a lane's eight elements (bf16/fp16: 16 bytes in x[0..3]; fp32: 32 bytes).
@@ -74,7 +75,7 @@ __device__ __forceinline__ Raw8<T> load_raw8(const T* __restrict__ slice, int n,
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (lane * 8 < n) v = __ldg(reinterpret_cast<const uint4*>(slice + lane * 8) + i);
+      if (vec_col<T>(lane, i) < n) v = __ldg(reinterpret_cast<const uint4*>(slice + vec_col<T>(lane, i)));
       r.x[4 * i] = v.x;
       r.x[4 * i + 1] = v.y;
       r.x[4 * i + 2] = v.z;
@@ -101,8 +102,8 @@ __device__ __forceinline__ void store_raw8(T* __restrict__ slice, int n, int lan
   if (kVec) {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      if (lane * 8 < n)
-        reinterpret_cast<uint4*>(slice + lane * 8)[i] =
+      if (vec_col<T>(lane, i) < n)
+        *reinterpret_cast<uint4*>(slice + vec_col<T>(lane, i)) =
             make_uint4(r.x[4 * i], r.x[4 * i + 1], r.x[4 * i + 2], r.x[4 * i + 3]);
   } else if (sizeof(T) == 4) {
     uint32_t* p = reinterpret_cast<uint32_t*>(slice);
@@ -145,6 +146,58 @@ __device__ __forceinline__ Raw8<T> from_floats(const float (&v)[8]) {
     for (int j = 0; j < 4; ++j) r.x[j] = pack2(v[2 * j], v[2 * j + 1], static_cast<const T*>(nullptr));
   }
   return r;
+}
+
+// Zeroes the rows that row_pair gives no pair: this block's share of them, as block
+// `part` of `parts`.  The shares are interleaved, because such rows come in runs (the
+// ends of the segments, the rest of the buffer): a block looks at every parts-th row,
+// a thread each, lists those without a pair in shared memory, and all its warps zero
+// the listed rows together, a slice each.  The whole block calls it.
+constexpr int kZeroList = 512;
+template <typename T, bool kVec>
+__device__ __forceinline__ void zero_rows(const int32_t* __restrict__ row_pair, int64_t pairs, int part, int parts, int R,
+                                          int H, T* __restrict__ rows) {
+  __shared__ int32_t list[kZeroList];
+  __shared__ int listed;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+  const int slices = (H + kSlice - 1) / kSlice;
+  const int per_pass = min(static_cast<int>(blockDim.x), kZeroList);
+  for (int64_t first = part; first < R; first += static_cast<int64_t>(per_pass) * parts) {
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    const int64_t r = first + static_cast<int64_t>(threadIdx.x) * parts;
+    if (static_cast<int>(threadIdx.x) < per_pass && r < R) {
+      const int p = row_pair[r];
+      if (p < 0 || p >= pairs) list[atomicAdd(&listed, 1)] = static_cast<int32_t>(r);
+    }
+    __syncthreads();
+    const int n = listed;
+    const Raw8<T> z = {};
+    int i = warp / slices, s = warp % slices;
+    for (; i < n;) {
+      store_raw8<T, kVec>(rows + static_cast<int64_t>(list[i]) * H + s * kSlice, H - s * kSlice, lane, z);
+      s += nwarp;
+      while (s >= slices) {
+        s -= slices;
+        ++i;
+      }
+    }
+    __syncthreads();   // the list is rewritten next
+  }
+}
+// Blocks for it behind a grid that does something else: two per SM, or one per 64 rows.
+inline unsigned zero_blocks_for(int R) { return static_cast<unsigned>(R < 64 * 296 ? (R + 63) / 64 : 296); }
+
+// Warps per token and tokens per block for `slices` slices of a row, two per warp.
+constexpr int kScatterWarps = 16;
+struct ScatterPlan {
+  int warps, tokens;
+};
+inline ScatterPlan plan_scatter(int slices) {
+  const int per = (slices + 1) / 2;
+  const int steps = (per + kScatterWarps - 1) / kScatterWarps;
+  const int warps = (per + steps - 1) / steps;
+  return ScatterPlan{warps, warps > 8 ? 1 : 8 / warps};
 }
 
 // Calls f(T*{}, bool_constant) for a dtype and access form.

@@ -37,41 +37,88 @@ __device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
   return e < -126 ? -126 : e;
 }
 
-// A slice of 256 columns = two blocks.  The vector form has a block per half-warp,
-// the other form every lane in both (elements 0..3 and 4..7).
-template <bool kVec>
-__device__ __forceinline__ void block_max(const uint32_t (&m)[2], uint32_t (&out)[2]) {
-  if (kVec) {
-    uint32_t v = max(m[0], m[1]);
+// Magnitudes as unsigned keys in the type's own bits: larger magnitude, larger
+// key; infinities and NaN are at least kOddKey.  Two 16-bit keys share a word.
+template <typename T>
+constexpr uint32_t kOddKey = 0x7f800000u;
+template <>
+constexpr uint32_t kOddKey<__nv_bfloat16> = 0x7f80u;
+template <>
+constexpr uint32_t kOddKey<__half> = 0x7c00u;
+
+__device__ __forceinline__ uint32_t key_bits(uint32_t key, const float*) { return key; }   // the magnitude's fp32 bits
+__device__ __forceinline__ uint32_t key_bits(uint32_t key, const __nv_bfloat16*) { return key << 16; }
+__device__ __forceinline__ uint32_t key_bits(uint32_t key, const __half*) {
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(key))));
+}
+
+// Largest key of elements 0..3 and of elements 4..7.
+template <typename T>
+__device__ __forceinline__ void max_keys(const Raw8<T>& r, uint32_t (&m)[2]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, off));
-    out[0] = out[1] = v;
+    for (int h = 0; h < 2; ++h)
+      m[h] = max(max(r.x[4 * h] & 0x7fffffffu, r.x[4 * h + 1] & 0x7fffffffu),
+                 max(r.x[4 * h + 2] & 0x7fffffffu, r.x[4 * h + 3] & 0x7fffffffu));
   } else {
-    out[0] = __reduce_max_sync(0xffffffffu, m[0]);
-    out[1] = __reduce_max_sync(0xffffffffu, m[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t k = __vmaxu2(r.x[2 * h] & 0x7fff7fffu, r.x[2 * h + 1] & 0x7fff7fffu);
+      m[h] = max(k & 0xffffu, k >> 16);
+    }
   }
 }
 
-// Codes (byte j = element j) and exponents of this lane's eight elements.
+// A slice of 256 columns = two blocks.  The vector form of 16-bit types has a block
+// per half-warp, the other forms every lane in both (elements 0..3 and 4..7).
 template <typename T, bool kVec>
-__device__ __forceinline__ uint2 encode8(const float (&v)[8], int (&e)[2]) {
-  uint32_t m[2] = {0u, 0u};
+constexpr bool kHalfWarp = kVec && sizeof(T) == 2;
+
+template <bool kHalf>
+__device__ __forceinline__ void block_max(uint32_t (&m)[2]) {
+  if (kHalf) {
+    uint32_t v = max(m[0], m[1]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m[j >> 2] = max(m[j >> 2], __float_as_uint(v[j]) & 0x7fffffffu);
-  uint32_t a[2];
-  block_max<kVec>(m, a);
-  const bool odd = max(a[0], a[1]) >= 0x7f800000u;
+    for (int off = 8; off >= 1; off >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, off));
+    m[0] = m[1] = v;
+  } else {
+    m[0] = __reduce_max_sync(0xffffffffu, m[0]);
+    m[1] = __reduce_max_sync(0xffffffffu, m[1]);
+  }
+}
+
+// The same for two sets of values, whose 16-bit keys go through the shuffles in one word.
+template <typename T, bool kVec>
+__device__ __forceinline__ void block_max2(uint32_t (&a)[2], uint32_t (&b)[2]) {
+  if constexpr (kHalfWarp<T, kVec>) {
+    uint32_t v = max(a[0], a[1]) | (max(b[0], b[1]) << 16);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, off));
+    a[0] = a[1] = v & 0xffffu;
+    b[0] = b[1] = v >> 16;
+  } else {
+    block_max<false>(a);
+    block_max<false>(b);
+  }
+}
+
+// Codes (byte j = element j) and exponents of this lane's eight elements, from their blocks' largest keys.
+template <typename T, bool kVec>
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], const uint32_t (&key)[2], int (&e)[2]) {
+  const T* type = nullptr;
+  uint32_t a[2] = {key_bits(key[0], type), key_bits(key[1], type)};
+  const bool odd = max(key[0], key[1]) >= kOddKey<T>;
   if (__any_sync(0xffffffffu, odd)) {   // a value that is not finite: the scale comes from the others
-    m[0] = m[1] = 0u;
+    a[0] = a[1] = 0u;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
-      if (b < 0x7f800000u) m[j >> 2] = max(m[j >> 2], b);
+      if (b < 0x7f800000u) a[j >> 2] = max(a[j >> 2], b);
     }
-    block_max<kVec>(m, a);
+    block_max<kHalfWarp<T, kVec>>(a);
   }
   e[0] = block_exponent(a[0]);
-  e[1] = block_exponent(a[1]);
+  e[1] = kHalfWarp<T, kVec> ? e[0] : block_exponent(a[1]);
   const float inv[2] = {pow2(-e[0]), pow2(-e[1])};
   float q[8];
 #pragma unroll
@@ -89,10 +136,13 @@ __device__ __forceinline__ uint2 encode8(const float (&v)[8], int (&e)[2]) {
   return make_uint2(pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7]));
 }
 
-template <bool kVec>
+template <typename T, bool kVec>
 __device__ __forceinline__ void store_codes(uint8_t* __restrict__ slice, int n, int lane, uint2 c) {
-  if (kVec) {
+  if (kHalfWarp<T, kVec>) {
     if (lane * 8 < n) *reinterpret_cast<uint2*>(slice + lane * 8) = c;
+  } else if (kVec) {
+    if (lane * 4 < n) *reinterpret_cast<uint32_t*>(slice + lane * 4) = c.x;
+    if (128 + lane * 4 < n) *reinterpret_cast<uint32_t*>(slice + 128 + lane * 4) = c.y;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -100,11 +150,14 @@ __device__ __forceinline__ void store_codes(uint8_t* __restrict__ slice, int n, 
   }
 }
 
-template <bool kVec>
+template <typename T, bool kVec>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* __restrict__ slice, int n, int lane) {
   uint2 c = make_uint2(0u, 0u);
-  if (kVec) {
+  if (kHalfWarp<T, kVec>) {
     if (lane * 8 < n) c = __ldg(reinterpret_cast<const uint2*>(slice + lane * 8));
+  } else if (kVec) {
+    if (lane * 4 < n) c.x = __ldg(reinterpret_cast<const uint32_t*>(slice + lane * 4));
+    if (128 + lane * 4 < n) c.y = __ldg(reinterpret_cast<const uint32_t*>(slice + 128 + lane * 4));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -114,26 +167,29 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* __restrict__ slice, i
 }
 
 // The slice's one or two exponent bytes.
-template <bool kVec>
+template <typename T, bool kVec>
 __device__ __forceinline__ void store_exponents(uint8_t* __restrict__ exps, int n, int lane, const int (&e)[2]) {
-  if (kVec) {
+  if (kHalfWarp<T, kVec>) {
     if ((lane & 15) == 0 && (lane >> 4) * kBlk < n) exps[lane >> 4] = static_cast<uint8_t>(e[0] + 127);
   } else {
-    if (lane < 2 && lane * kBlk < n) exps[lane] = static_cast<uint8_t>(e[lane] + 127);
+    if (lane < 2 && lane * kBlk < n) exps[lane] = static_cast<uint8_t>((lane ? e[1] : e[0]) + 127);
   }
 }
 
-// The values of eight codes (in [0, 448], exact) times their blocks' scales.
-template <bool kVec>
-__device__ __forceinline__ void decode8(uint2 c, const uint8_t* __restrict__ exps, int n, int lane, float (&v)[8]) {
-  float s[2];
-  if (kVec) {
+// 2^e of this lane's two blocks (of the one that it is in, twice, where a half-warp has a block).
+template <typename T, bool kVec>
+__device__ __forceinline__ void load_scales(const uint8_t* __restrict__ exps, int n, int lane, float (&s)[2]) {
+  if (kHalfWarp<T, kVec>) {
     const int b = lane >> 4;
     s[0] = s[1] = b * kBlk < n ? __uint_as_float(static_cast<uint32_t>(__ldg(exps + b)) << 23) : 0.f;
   } else {
-    s[0] = __uint_as_float(static_cast<uint32_t>(__ldg(exps)) << 23);
+    s[0] = 0 < n ? __uint_as_float(static_cast<uint32_t>(__ldg(exps)) << 23) : 0.f;
     s[1] = kBlk < n ? __uint_as_float(static_cast<uint32_t>(__ldg(exps + 1)) << 23) : 0.f;
   }
+}
+
+// The values of eight codes times their blocks' scales, exact in fp32.
+__device__ __forceinline__ void decode8(uint2 c, const float (&s)[2], float (&v)[8]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t w = (j < 2 ? c.x : c.y) >> (16 * (j & 1));
@@ -143,47 +199,132 @@ __device__ __forceinline__ void decode8(uint2 c, const uint8_t* __restrict__ exp
   }
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// 1 / (1 + e^-x), both steps within 2 ulp; 0 where 1 + e^-x is beyond 2^126.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
 
-// One warp per (row, slice).
+// One warp per (row, group of kGroup slices), consecutive warps on consecutive
+// groups of a row: this warp's row and first slice.
+struct Unit {
+  int64_t row;
+  int slice;
+};
+template <int kGroup>
+__device__ __forceinline__ Unit unit_of(int slices) {
+  const unsigned groups = (slices + kGroup - 1) / kGroup;
+  const unsigned u = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  return Unit{u / groups, static_cast<int>(u % groups) * kGroup};
+}
+
+// Slices per warp whose loads are in flight together.
+constexpr int kPackGroup = 4;
+constexpr int kRestoreGroup = 4;
+template <typename T>
+constexpr int kSwigluGroup = sizeof(T) == 4 ? 1 : 2;
+
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t stride, int R, int W,
                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   const int lane = threadIdx.x & 31;
   const int slices = (W + kSlice - 1) / kSlice, nb = (W + kBlk - 1) / kBlk;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t r = u / slices;
-  if (r >= R) return;
-  const int c = static_cast<int>(u % slices) * kSlice, n = W - c;
-  float v[8];
-  to_floats(load_raw8<T, kVec>(x + r * stride + c, n, lane), v);
-  int e[2];
-  const uint2 q = encode8<T, kVec>(v, e);
-  store_codes<kVec>(codes + r * W + c, n, lane, q);
-  store_exponents<kVec>(exps + r * nb + c / kBlk, n, lane, e);
+  const Unit u = unit_of<kPackGroup>(slices);
+  if (u.row >= R) return;
+  const T* src = x + u.row * stride;
+  Raw8<T> raw[kPackGroup];
+#pragma unroll
+  for (int j = 0; j < kPackGroup; ++j) {
+    const int c = (u.slice + j) * kSlice;
+    raw[j] = load_raw8<T, kVec>(src + c, W - c, lane);   // past the width: nothing is read
+  }
+#pragma unroll
+  for (int j = 0; j < kPackGroup; ++j) {
+    const int c = (u.slice + j) * kSlice, n = W - c;
+    if (n <= 0) break;
+    float v[8];
+    uint32_t key[2];
+    int e[2];
+    max_keys(raw[j], key);
+    block_max<kHalfWarp<T, kVec>>(key);
+    to_floats(raw[j], v);
+    const uint2 q = encode8<T, kVec>(v, key, e);
+    store_codes<T, kVec>(codes + u.row * W + c, n, lane, q);
+    store_exponents<T, kVec>(exps + u.row * nb + c / kBlk, n, lane, e);
+  }
 }
 
-// One warp per (row, slice); with row_pair, output row i is the row of pair row_pair[i] (zeros if it has none).
+template <typename T, bool kVec>
+__device__ __forceinline__ Raw8<T> restored(uint2 codes, const float (&s)[2]) {
+  float v[8];
+  decode8(codes, s, v);
+  return from_floats<T>(v);
+}
+
+// Rows as they were.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __restrict__ codes,
-                                                            const uint8_t* __restrict__ exps, int src_rows, int W,
-                                                            const int32_t* __restrict__ row_pair, int K, int R,
+                                                            const uint8_t* __restrict__ exps, int R, int W,
                                                             T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   const int slices = (W + kSlice - 1) / kSlice, nb = (W + kBlk - 1) / kBlk;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t r = u / slices;
-  if (r >= R) return;
-  const int c = static_cast<int>(u % slices) * kSlice, n = W - c;
-  int64_t src = r;
-  if (row_pair) {
-    const int p = row_pair[r];
-    src = p >= 0 ? p / K : -1;
+  const Unit u = unit_of<kRestoreGroup>(slices);
+  if (u.row >= R) return;
+  uint2 q[kRestoreGroup];
+  float s[kRestoreGroup][2];
+#pragma unroll
+  for (int j = 0; j < kRestoreGroup; ++j) {
+    const int c = (u.slice + j) * kSlice;
+    q[j] = load_codes<T, kVec>(codes + u.row * W + c, W - c, lane);
+    load_scales<T, kVec>(exps + u.row * nb + c / kBlk, W - c, lane, s[j]);
   }
-  float v[8] = {};
-  if (src >= 0 && src < src_rows)
-    decode8<kVec>(load_codes<kVec>(codes + src * W + c, n, lane), exps + src * nb + c / kBlk, n, lane, v);
-  store_raw8<T, kVec>(out + r * W + c, n, lane, from_floats<T>(v));
+#pragma unroll
+  for (int j = 0; j < kRestoreGroup; ++j) {
+    const int c = (u.slice + j) * kSlice;
+    store_raw8<T, kVec>(out + u.row * W + c, W - c, lane, restored<T, kVec>(q[j], s[j]));
+  }
+}
+
+// Rows in expert order: a block holds a token's row across its warps, two slices
+// each, decodes it once and stores it K times (as scatter_rows_kernel, whose reason
+// for one block per token holds here too).  Blocks past the tokens zero the rows of
+// no pair.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
+    const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int T_, int W,
+    const int32_t* __restrict__ pair_row, const int32_t* __restrict__ row_pair, int K, int R, int warps, int tokens,
+    unsigned token_blocks, T* __restrict__ out) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x >= token_blocks) {
+    zero_rows<T, kVec>(row_pair, static_cast<int64_t>(T_) * K, blockIdx.x - token_blocks, gridDim.x - token_blocks, R, W,
+                       out);
+    return;
+  }
+  const int sub = warp / warps;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + sub;
+  if (t >= T_) return;
+  const int nb = (W + kBlk - 1) / kBlk;
+  int mine = -1;
+  if (lane < K) mine = pair_row[t * K + lane];
+  for (int c0 = (warp - sub * warps) * kSlice; c0 < W; c0 += 2 * warps * kSlice) {
+    uint2 q[2];
+    float s[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c = c0 + j * warps * kSlice;
+      q[j] = load_codes<T, kVec>(codes + t * W + c, W - c, lane);
+      load_scales<T, kVec>(exps + t * nb + c / kBlk, W - c, lane, s[j]);
+    }
+    Raw8<T> v[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = restored<T, kVec>(q[j], s[j]);
+    for (int k = 0; k < K; ++k) {
+      const int row = __shfl_sync(0xffffffffu, mine, k);
+      if (row < 0 || row >= R) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = c0 + j * warps * kSlice;
+        store_raw8<T, kVec>(out + static_cast<int64_t>(row) * W + c, W - c, lane, v[j]);
+      }
+    }
+  }
 }
 
 // h = [up | gate]: act = up * silu(gate), and h kept in 8 bits (each half's blocks begin at its own column 0).
@@ -191,27 +332,44 @@ template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restrict__ h, int64_t stride, int R, int I,
                                                                 T* __restrict__ act, uint8_t* __restrict__ codes,
                                                                 uint8_t* __restrict__ exps) {
+  constexpr int kGroup = kSwigluGroup<T>;
   const int lane = threadIdx.x & 31;
   const int slices = (I + kSlice - 1) / kSlice, nb = (I + kBlk - 1) / kBlk;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t r = unit / slices;
-  if (r >= R) return;
-  const int c = static_cast<int>(unit % slices) * kSlice, n = I - c;
-  float u[8], g[8], a[8];
-  to_floats(load_raw8<T, kVec>(h + r * stride + c, n, lane), u);
-  to_floats(load_raw8<T, kVec>(h + r * stride + I + c, n, lane), g);
+  const Unit unit = unit_of<kGroup>(slices);
+  if (unit.row >= R) return;
+  const int64_t r = unit.row;
+  Raw8<T> ru[kGroup], rg[kGroup];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = u[j] * (g[j] * sigmoid(g[j]));
-  store_raw8<T, kVec>(act + r * I + c, n, lane, from_floats<T>(a));
-  uint8_t* cr = codes + r * 2 * I + c;
-  uint8_t* er = exps + r * 2 * nb + c / kBlk;
-  int e[2];
-  uint2 q = encode8<T, kVec>(u, e);
-  store_codes<kVec>(cr, n, lane, q);
-  store_exponents<kVec>(er, n, lane, e);
-  q = encode8<T, kVec>(g, e);
-  store_codes<kVec>(cr + I, n, lane, q);
-  store_exponents<kVec>(er + nb, n, lane, e);
+  for (int i = 0; i < kGroup; ++i) {
+    const int c = (unit.slice + i) * kSlice, n = I - c;
+    ru[i] = load_raw8<T, kVec>(h + r * stride + c, n, lane);
+    rg[i] = load_raw8<T, kVec>(h + r * stride + I + c, n, lane);
+  }
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    const int c = (unit.slice + i) * kSlice, n = I - c;
+    if (n <= 0) break;
+    float u[8], g[8], a[8];
+    to_floats(ru[i], u);
+    to_floats(rg[i], g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = u[j] * (g[j] * sigmoid(g[j]));
+    store_raw8<T, kVec>(act + r * I + c, n, lane, from_floats<T>(a));
+    if (!codes) continue;   // the activation alone
+    uint32_t ku[2], kg[2];
+    max_keys(ru[i], ku);
+    max_keys(rg[i], kg);
+    block_max2<T, kVec>(ku, kg);
+    uint8_t* cr = codes + r * 2 * I + c;
+    uint8_t* er = exps + r * 2 * nb + c / kBlk;
+    int e[2];
+    uint2 q = encode8<T, kVec>(u, ku, e);
+    store_codes<T, kVec>(cr, n, lane, q);
+    store_exponents<T, kVec>(er, n, lane, e);
+    q = encode8<T, kVec>(g, kg, e);
+    store_codes<T, kVec>(cr + I, n, lane, q);
+    store_exponents<T, kVec>(er + nb, n, lane, e);
+  }
 }
 
 // From the kept values u, g and d = dL/dact: du = d g s, dg = d u s (1 + g (1 - s)), act = u g s, with s = sigmoid(g).
@@ -220,40 +378,58 @@ __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_
                                                                     const uint8_t* __restrict__ exps,
                                                                     const T* __restrict__ grad, int64_t stride, int R,
                                                                     int I, T* __restrict__ dh, T* __restrict__ act) {
+  constexpr int kGroup = kSwigluGroup<T>;
   const int lane = threadIdx.x & 31;
   const int slices = (I + kSlice - 1) / kSlice, nb = (I + kBlk - 1) / kBlk;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t r = unit / slices;
-  if (r >= R) return;
-  const int c = static_cast<int>(unit % slices) * kSlice, n = I - c;
-  float u[8], g[8], d[8], a[8];
-  const uint8_t* cr = codes + r * 2 * I + c;
-  const uint8_t* er = exps + r * 2 * nb + c / kBlk;
-  to_floats(load_raw8<T, kVec>(grad + r * stride + c, n, lane), d);
-  decode8<kVec>(load_codes<kVec>(cr, n, lane), er, n, lane, u);
-  decode8<kVec>(load_codes<kVec>(cr + I, n, lane), er + nb, n, lane, g);
+  const Unit unit = unit_of<kGroup>(slices);
+  if (unit.row >= R) return;
+  const int64_t r = unit.row;
+  Raw8<T> rd[kGroup];
+  uint2 qu[kGroup], qg[kGroup];
+  float su[kGroup][2], sg[kGroup][2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float s = sigmoid(g[j]);
-    const float gs = g[j] * s;
-    a[j] = u[j] * gs;
-    const float dg = d[j] * (u[j] * s * (1.0f + g[j] * (1.0f - s)));
-    u[j] = d[j] * gs;
-    g[j] = dg;
+  for (int i = 0; i < kGroup; ++i) {
+    const int c = (unit.slice + i) * kSlice, n = I - c;
+    const uint8_t* cr = codes + r * 2 * I + c;
+    const uint8_t* er = exps + r * 2 * nb + c / kBlk;
+    rd[i] = load_raw8<T, kVec>(grad + r * stride + c, n, lane);
+    qu[i] = load_codes<T, kVec>(cr, n, lane);
+    qg[i] = load_codes<T, kVec>(cr + I, n, lane);
+    load_scales<T, kVec>(er, n, lane, su[i]);
+    load_scales<T, kVec>(er + nb, n, lane, sg[i]);
   }
-  store_raw8<T, kVec>(dh + r * 2 * I + c, n, lane, from_floats<T>(u));
-  store_raw8<T, kVec>(dh + r * 2 * I + I + c, n, lane, from_floats<T>(g));
-  if (act) store_raw8<T, kVec>(act + r * I + c, n, lane, from_floats<T>(a));
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    const int c = (unit.slice + i) * kSlice, n = I - c;
+    if (n <= 0) break;
+    float u[8], g[8], d[8], a[8];
+    to_floats(rd[i], d);
+    decode8(qu[i], su[i], u);
+    decode8(qg[i], sg[i], g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = sigmoid(g[j]);
+      const float gs = g[j] * s;
+      a[j] = u[j] * gs;
+      const float dg = d[j] * (u[j] * s * (1.0f + g[j] * (1.0f - s)));
+      u[j] = d[j] * gs;
+      g[j] = dg;
+    }
+    store_raw8<T, kVec>(dh + r * 2 * I + c, n, lane, from_floats<T>(u));
+    store_raw8<T, kVec>(dh + r * 2 * I + I + c, n, lane, from_floats<T>(g));
+    if (act) store_raw8<T, kVec>(act + r * I + c, n, lane, from_floats<T>(a));
+  }
 }
 
 bool valid_rows(int64_t R, int64_t W, int32_t dtype) {
   return R >= 0 && R <= KF_SORT_MAX_ROWS && W >= 1 && W <= KF_SORT_MAX_WIDTH && valid_dtype(dtype);
 }
 
-// Blocks of a grid of one warp per (row, slice); 0 when they are more than a grid holds.
-unsigned grid_of(int64_t R, int64_t W) {
-  const int64_t b = (R * ((W + kSlice - 1) / kSlice) + kWarps - 1) / kWarps;
-  return b <= 0x7fffffff ? static_cast<unsigned>(b) : 0u;
+// Blocks of a grid of one warp per (row, group of slices); 0 when they are too many (rows of terabytes).
+unsigned grid_of(int64_t R, int64_t W, int group) {
+  const int64_t slices = (W + kSlice - 1) / kSlice;
+  const int64_t units = R * ((slices + group - 1) / group);
+  return units <= 0xffffffffll - kWarps ? static_cast<unsigned>((units + kWarps - 1) / kWarps) : 0u;
 }
 
 inline bool aligned(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -285,7 +461,7 @@ int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, i
              void* exponents, void* stream) {
   if (!valid_rows(num_rows, width, dtype) || x_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, width);
+  const unsigned grid = grid_of(num_rows, width, kPackGroup);
   if (!x || !codes || !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(x, x_stride, width, dtype) && aligned(codes, 8);
   return launch(dtype, vec, [&](auto t, auto v) {
@@ -297,18 +473,32 @@ int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, i
 }
 
 int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t num_rows, int32_t width,
-                const int32_t* row_pair, int32_t top_k, int32_t out_rows, void* output, void* stream) {
+                const int32_t* pair_row, const int32_t* row_pair, int32_t top_k, int32_t out_rows, void* output,
+                void* stream) {
   if (!valid_rows(num_rows, width, dtype) || !valid_rows(out_rows, width, dtype)) return KF_ERR_INVALID_ARGUMENT;
-  if (row_pair ? (top_k < 1 || top_k > KF_SORT_MAX_TOP_K) : out_rows != num_rows) return KF_ERR_INVALID_ARGUMENT;
+  if (num_rows > 0 && (!codes || !exponents)) return KF_ERR_INVALID_ARGUMENT;
+  const bool sorted = row_pair != nullptr;
+  if (sorted ? (top_k < 1 || top_k > KF_SORT_MAX_TOP_K || !valid_tokens(num_rows) || (num_rows > 0 && !pair_row))
+             : out_rows != num_rows)
+    return KF_ERR_INVALID_ARGUMENT;
   if (out_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(out_rows, width);
-  if (!output || !grid || (num_rows > 0 && (!codes || !exponents))) return KF_ERR_INVALID_ARGUMENT;
+  const unsigned grid = grid_of(num_rows, width, kRestoreGroup);
+  if (!output || (num_rows > 0 && !grid)) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(output, width, width, dtype) && aligned(codes, 8);
   return launch(dtype, vec, [&](auto t, auto v) {
     using E = ElemOf<decltype(t)>;
-    restore8_kernel<E, decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(exponents), num_rows, width, row_pair, top_k,
-        out_rows, static_cast<E*>(output));
+    const uint8_t* c = static_cast<const uint8_t*>(codes);
+    const uint8_t* e = static_cast<const uint8_t*>(exponents);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (sorted) {
+      const ScatterPlan p = plan_scatter((width + kSlice - 1) / kSlice);
+      const unsigned nwarp = p.warps * p.tokens, token_blocks = (num_rows + p.tokens - 1) / p.tokens;
+      restore8_sorted_kernel<E, decltype(v)::value><<<token_blocks + zero_blocks_for(out_rows), nwarp * 32, 0, s>>>(
+          c, e, num_rows, width, pair_row, row_pair, top_k, out_rows, p.warps, p.tokens, token_blocks,
+          static_cast<E*>(output));
+    } else {
+      restore8_kernel<E, decltype(v)::value><<<grid, kThreads, 0, s>>>(c, e, num_rows, width, static_cast<E*>(output));
+    }
   });
 }
 
@@ -316,8 +506,8 @@ int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_
                     void* codes, void* exponents, void* stream) {
   if (!valid_rows(num_rows, inter, dtype) || h_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, inter);
-  if (!h || !act || !codes || !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
+  const unsigned grid = grid_of(num_rows, inter, dtype == KF_DTYPE_F32 ? kSwigluGroup<float> : kSwigluGroup<__half>);
+  if (!h || !act || !codes != !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(h, h_stride, inter, dtype) && vec_rows(act, inter, inter, dtype) && aligned(codes, 8);
   return launch(dtype, vec, [&](auto t, auto v) {
     using E = ElemOf<decltype(t)>;
@@ -331,7 +521,7 @@ int kf_swiglu_backward8(const void* codes, const void* exponents, const void* gr
                         int64_t grad_stride, int32_t num_rows, int32_t inter, void* grad_h, void* act, void* stream) {
   if (!valid_rows(num_rows, inter, dtype) || grad_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, inter);
+  const unsigned grid = grid_of(num_rows, inter, dtype == KF_DTYPE_F32 ? kSwigluGroup<float> : kSwigluGroup<__half>);
   if (!codes || !exponents || !grad_act || !grad_h || !grid) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(grad_act, grad_stride, inter, dtype) && vec_rows(grad_h, inter, inter, dtype) &&
                    (!act || vec_rows(act, inter, inter, dtype)) && aligned(codes, 8);

@@ -11,29 +11,48 @@
 //
 // The reference sorts and combines inside its kernel() only, for its own FP8
 // layer and without gradients (solution/triton/kernel.py:46-82, :1920-1925).
+#include <algorithm>
+
 #include "kf_elem.cuh"
 #include "kf_internal.cuh"
+#include "kf_ptx.cuh"
 
 namespace kf {
 namespace {
 
-constexpr int kOrderThreads = 256;
-constexpr int kOrderChunk = 1024;   // pairs per chunk of the counting sort
-constexpr int kRowThreads = 256;
-constexpr int kWarps = kRowThreads / 32;
+constexpr int kPlaceThreads = 1024;
+constexpr int kPlaceWarps = kPlaceThreads / 32;
+constexpr int kHistThreads = 256;
+constexpr int kMaxChunks = 128;      // histogram chunks of a large call: what each block of the placing kernel sums
+constexpr int kDirectPairs = 8192;   // calls of at most this many pairs need no histogram kernel
 
 __device__ __forceinline__ int local_expert(int id, int offset, int E) {
   const unsigned le = static_cast<unsigned>(id) - static_cast<unsigned>(offset);
   return id >= 0 && le < static_cast<unsigned>(E) ? static_cast<int>(le) : -1;
 }
 
-__global__ void __launch_bounds__(kOrderThreads) order_hist_kernel(const int32_t* __restrict__ ids, int n, int E,
-                                                                   int offset, int32_t* __restrict__ hist) {
+// Tokens per histogram chunk, and chunks (0: the placing kernel counts the pairs itself).
+struct OrderPlan {
+  int chunk_tokens, nchunk;
+};
+
+inline OrderPlan plan_order(int T, int K) {
+  if (static_cast<int64_t>(T) * K <= kDirectPairs) return OrderPlan{T, 0};
+  const int least = (1024 + K - 1) / K, even = (T + kMaxChunks - 1) / kMaxChunks;
+  const int ct = least > even ? least : even;
+  return OrderPlan{ct, (T + ct - 1) / ct};
+}
+
+// hist[c][e] = pairs of local expert e among the tokens of chunk c.
+__global__ void __launch_bounds__(kHistThreads) order_hist_kernel(const int32_t* __restrict__ ids, int n, int E,
+                                                                  int offset, int chunk_pairs,
+                                                                  int32_t* __restrict__ hist) {
+  grid_dep_trigger();
   __shared__ int32_t h[kEG];
   h[threadIdx.x] = 0;
   __syncthreads();
-  const int p0 = blockIdx.x * kOrderChunk;
-  for (int p = p0 + threadIdx.x; p < min(n, p0 + kOrderChunk); p += kOrderThreads) {
+  const int p0 = blockIdx.x * chunk_pairs, p1 = min(n, p0 + chunk_pairs);
+  for (int p = p0 + threadIdx.x; p < p1; p += kHistThreads) {
     const int e = local_expert(ids[p], offset, E);
     if (e >= 0) atomicAdd(&h[e], 1);
   }
@@ -41,181 +60,611 @@ __global__ void __launch_bounds__(kOrderThreads) order_hist_kernel(const int32_t
   if (threadIdx.x < E) hist[static_cast<size_t>(blockIdx.x) * E + threadIdx.x] = h[threadIdx.x];
 }
 
-// One block; thread e owns expert e.  hist[c][e] becomes the row of the first pair of expert e in chunk c.
-__global__ void __launch_bounds__(kOrderThreads) order_scan_kernel(int32_t* __restrict__ hist, int nchunk, int E,
-                                                                   int align, int rows, int32_t* __restrict__ counts,
-                                                                   int32_t* __restrict__ starts) {
-  __shared__ int64_t scan[kOrderThreads];
-  const int e = threadIdx.x;
-  int run = 0;
-  if (e < E)
-    for (int c = 0; c < nchunk; ++c) run += hist[static_cast<size_t>(c) * E + e];
-  const int64_t padded = (static_cast<int64_t>(run) + align - 1) / align * align;
-  scan[e] = padded;
-  __syncthreads();
-  for (int off = 1; off < kOrderThreads; off <<= 1) {
-    const int64_t v = e >= off ? scan[e - off] : 0;
-    __syncthreads();
-    scan[e] += v;
-    __syncthreads();
-  }
-  if (e >= E) return;
-  const int64_t start = scan[e] - padded;
-  counts[e] = run;
-  starts[e] = static_cast<int32_t>(start < rows ? start : rows);
-  if (e == E - 1) starts[E] = static_cast<int32_t>(scan[e] < rows ? scan[e] : rows);
-  // past the buffer every pair is dropped, so a start there only has to stay past it
-  int at = static_cast<int32_t>(start < rows ? start : rows);
-  for (int c = 0; c < nchunk; ++c) {
-    const int k = hist[static_cast<size_t>(c) * E + e];
-    hist[static_cast<size_t>(c) * E + e] = at;
-    at = at > rows - k ? rows : at + k;
-  }
-}
+struct PlaceArgs {
+  const int32_t* ids;
+  const int32_t* hist;   // [nchunk][E]
+  int T, K, H, E, offset, align, R;
+  int chunk_tokens, nchunk;
+  int64_t stride;        // elements between rows of x
+  int32_t *pair_row, *row_pair, *counts, *starts;
+};
 
-__global__ void __launch_bounds__(kOrderThreads) order_place_kernel(const int32_t* __restrict__ ids, int n, int E,
-                                                                    int offset, const int32_t* __restrict__ first,
-                                                                    int rows, int32_t* __restrict__ pair_row,
-                                                                    int32_t* __restrict__ row_pair) {
-  __shared__ int32_t at[kEG];                          // next row of each expert
-  __shared__ int32_t warp_count[kOrderThreads / 32][kEG];
+// Places and copies: block b owns the tokens [b T / G, (b + 1) T / G).
+//
+// Counting.  Each block finds, for every expert, the pairs of the whole call and
+// those before its own first token: from the histogram's rows and the ids between
+// the last chunk border and its first token, or in small calls from all ids.  So
+// no block waits for another, and the order needs one launch or two.
+// Ranks.  A pair's row is its expert's next row, plus the pairs of its expert in
+// the block's earlier warps, plus those in lower lanes of its own warp: stable and
+// without atomics on the order.
+// Rows (kCopy; small calls, where one launch is worth more than the last of the
+// bandwidth).  Each token's row is read once and stored once per pair, 256 columns
+// per warp and step, four steps' loads in flight.  Rows that no pair has -- the
+// ends of the segments and the rest of the buffer -- are shared by all blocks.
+template <typename T, bool kVec, bool kCopy>
+__global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const PlaceArgs a, const T* __restrict__ x,
+                                                                        T* __restrict__ rows) {
+  if (!kCopy) grid_dep_trigger();
+  __shared__ int32_t total[kEG], before[kEG];        // before becomes the next row of each expert
+  __shared__ int32_t zero_first[kEG + 1];            // first row of expert e's padding; the last entry: the buffer's rest
+  __shared__ int32_t zero_upto[kEG + 1];             // padding rows of experts <= e
+  __shared__ uint16_t warp_count[kPlaceWarps][kEG];
+  __shared__ int32_t srow[kPlaceThreads];
+  __shared__ int32_t warp_sum[2][kEG / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  at[tid] = tid < E ? first[static_cast<size_t>(blockIdx.x) * E + tid] : 0;
-  const int p0 = blockIdx.x * kOrderChunk;
-  for (int r = 0; r < kOrderChunk; r += kOrderThreads) {
-    for (int w = 0; w < kOrderThreads / 32; ++w) warp_count[w][tid] = 0;
-    __syncthreads();
-    const int p = p0 + r + tid;
-    const int e = p < n ? local_expert(ids[p], offset, E) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int before = __popc(same & ((1u << lane) - 1u));
-    if (e >= 0 && before == 0) warp_count[warp][e] = __popc(same);
-    __syncthreads();
-    int row = -1;
-    if (e >= 0) {
-      row = at[e] + before;
-      for (int w = 0; w < warp; ++w) row += warp_count[w][e];
+  const int G = gridDim.x;
+  const int t0 = static_cast<int>(static_cast<int64_t>(a.T) * blockIdx.x / G);
+  const int t1 = static_cast<int>(static_cast<int64_t>(a.T) * (blockIdx.x + 1) / G);
+
+  if (tid < kEG) total[tid] = before[tid] = 0;
+  __syncthreads();
+  const int first_pair = t0 * a.K;
+  if (a.nchunk == 0) {
+    const int n = a.T * a.K;
+    for (int p = tid; p < n; p += kPlaceThreads) {
+      const int e = local_expert(a.ids[p], a.offset, a.E);
+      if (e >= 0) {
+        atomicAdd(&total[e], 1);
+        if (p < first_pair) atomicAdd(&before[e], 1);
+      }
     }
-    if (p < n) {
-      if (row >= rows) row = -1;
-      pair_row[p] = row;
-      if (row >= 0) row_pair[row] = p;
+  } else {
+    const int c0 = t0 / a.chunk_tokens;
+    for (int p = c0 * a.chunk_tokens * a.K + tid; p < first_pair; p += kPlaceThreads) {
+      const int e = local_expert(a.ids[p], a.offset, a.E);
+      if (e >= 0) atomicAdd(&before[e], 1);
+    }
+    grid_dep_wait();   // the histogram is complete
+    const int e = tid & (kEG - 1);
+    if (e < a.E) {
+      int all = 0, bef = 0;
+#pragma unroll 8
+      for (int c = tid / kEG; c < a.nchunk; c += kPlaceThreads / kEG) {
+        const int v = a.hist[static_cast<size_t>(c) * a.E + e];
+        all += v;
+        if (c < c0) bef += v;
+      }
+      atomicAdd(&total[e], all);
+      atomicAdd(&before[e], bef);
+    }
+  }
+  __syncthreads();
+
+  // segments: inclusive scan of the padded counts over the experts, and of the padding inside the buffer
+  int count = 0, padded = 0, incl = 0;
+  if (tid < kEG) {
+    count = total[tid];
+    padded = (count + a.align - 1) / a.align * a.align;
+    incl = padded;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
+    }
+    if (lane == 31) warp_sum[0][warp] = incl;
+  }
+  __syncthreads();
+  int pads = 0, pads_incl = 0;
+  if (tid < kEG) {
+    for (int w = 0; w < warp; ++w) incl += warp_sum[0][w];
+    const int start = incl - padded;
+    before[tid] += start;
+    const int live_end = min(start + count, a.R), end = min(incl, a.R);
+    pads = end - live_end;
+    zero_first[tid] = live_end;
+    if (blockIdx.x == 0 && tid < a.E) {
+      a.counts[tid] = count;
+      a.starts[tid] = min(start, a.R);
+      if (tid == a.E - 1) a.starts[a.E] = end;
+    }
+    if (tid == kEG - 1) zero_first[kEG] = end;   // experts past E have no rows: the last one ends them all
+    pads_incl = pads;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, pads_incl, off);
+      if (lane >= off) pads_incl += v;
+    }
+    if (lane == 31) warp_sum[1][warp] = pads_incl;
+  }
+  __syncthreads();
+  if (tid < kEG) {
+    for (int w = 0; w < warp; ++w) pads_incl += warp_sum[1][w];
+    zero_upto[tid] = pads_incl;
+    if (tid == kEG - 1) zero_upto[kEG] = pads_incl + a.R - zero_first[kEG];
+  }
+
+  const int slices = (a.H + kSlice - 1) / kSlice;
+  const int round_tokens = kPlaceThreads / a.K;
+  for (int r0 = t0; r0 < t1; r0 += round_tokens) {
+    const int ntok = min(round_tokens, t1 - r0), npair = ntok * a.K;
+    const int nwarp = (npair + 31) / 32;
+    for (int i = tid; i < nwarp * (kEG / 2); i += kPlaceThreads) reinterpret_cast<uint32_t*>(warp_count)[i] = 0u;
+    __syncthreads();   // also: zero_upto, before, and the previous round's reads of srow
+    const int p = r0 * a.K + tid;
+    int e = -1, rank = 0;
+    if (warp < nwarp) {
+      e = tid < npair ? local_expert(a.ids[p], a.offset, a.E) : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      rank = __popc(same & ((1u << lane) - 1u));
+      if (e >= 0 && rank == 0) warp_count[warp][e] = static_cast<uint16_t>(__popc(same));
     }
     __syncthreads();
-    int sum = 0;
-    for (int w = 0; w < kOrderThreads / 32; ++w) sum += warp_count[w][tid];
-    at[tid] += sum;
+    if (tid < kEG) {   // counts become the pairs in earlier warps; `before` moves on after the rows are read
+      int run = 0;
+      for (int w = 0; w < nwarp; ++w) {
+        const int v = warp_count[w][tid];
+        warp_count[w][tid] = static_cast<uint16_t>(run);
+        run += v;
+      }
+      total[tid] = run;   // this round's pairs
+    }
     __syncthreads();
-  }
-}
+    if (tid < npair) {
+      int row = -1;
+      if (e >= 0) {
+        row = before[e] + warp_count[warp][e] + rank;
+        if (row >= a.R) row = -1;
+      }
+      srow[tid] = row;
+      a.pair_row[p] = row;
+      if (row >= 0) a.row_pair[row] = p;
+    }
+    __syncthreads();
+    if (tid < kEG) before[tid] += total[tid];
 
-// One warp per row of the buffer, 16-byte (or single-element) accesses.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) gather_tokens_kernel(const T* __restrict__ x, int64_t stride, int T_,
-                                                                    int K, int H, const int32_t* __restrict__ row_pair,
-                                                                    int rows, T* __restrict__ out) {
-  const int lane = threadIdx.x & 31;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  const int p = row_pair[r];
-  const int t = p >= 0 ? p / K : -1;
-  const bool live = t >= 0 && t < T_;
-  const T* src = x + (live ? static_cast<int64_t>(t) * stride : 0);
-  T* dst = out + r * H;
-  for (int c = 0; c < H; c += kSlice) {
-    const Raw8<T> v = load_raw8<T, kVec>(src + c, live ? H - c : 0, lane);
-    store_raw8<T, kVec>(dst + c, H - c, lane, v);
-  }
-}
-
-// One warp per (token, slice of 256 columns); lane k of the warp holds pair k's row and weight.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) combine_kernel(const T* __restrict__ rows, int64_t stride, int R,
-                                                              const int32_t* __restrict__ pair_row,
-                                                              const float* __restrict__ weight, int T_, int K, int H,
-                                                              T* __restrict__ out) {
-  const int lane = threadIdx.x & 31;
-  const int slices = (H + kSlice - 1) / kSlice;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t t = u / slices;
-  if (t >= T_) return;
-  const int c = static_cast<int>(u % slices) * kSlice;
-  int my_row = -1;
-  float my_w = 1.f;
-  if (lane < K) {
-    my_row = pair_row[t * K + lane];
-    if (my_row >= R) my_row = -1;
-    if (weight) my_w = weight[t * K + lane];
-  }
-  float acc[8] = {};
-  for (int k = 0; k < K; ++k) {
-    const int row = __shfl_sync(0xffffffffu, my_row, k);
-    const float w = __shfl_sync(0xffffffffu, my_w, k);
-    if (row < 0) continue;
-    float v[8];
-    to_floats(load_raw8<T, kVec>(rows + static_cast<int64_t>(row) * stride + c, H - c, lane), v);
+    if constexpr (!kCopy) continue;
+    const int units = ntok * slices;
+    constexpr int kStep = 4;
+    int i = warp / slices, sl = warp % slices;   // this warp's next unit: token r0 + i, slice sl
+    for (int u = warp; u < units; u += kStep * kPlaceWarps) {
+      Raw8<T> v[kStep];
+      int ti[kStep], tc[kStep];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, v[j], acc[j]);
-  }
-  store_raw8<T, kVec>(out + t * H + c, H - c, lane, from_floats<T>(acc));
-}
-
-// Blocks [0, T): one per token.  Blocks past T: rows without a pair are zeroed.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) combine_backward_kernel(
-    const T* __restrict__ dout, const T* __restrict__ rows, int64_t stride, int R, const int32_t* __restrict__ pair_row,
-    const int32_t* __restrict__ row_pair, const float* __restrict__ weight, int T_, int K, int H, T* __restrict__ drows,
-    float* __restrict__ dweight) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x >= T_) {
-    if (!drows) return;
-    const int64_t r = static_cast<int64_t>(blockIdx.x - T_) * kWarps + warp;
-    if (r >= R) return;
-    const int p = row_pair[r];
-    if (p >= 0 && p < static_cast<int64_t>(T_) * K) return;
-    Raw8<T> z = {};
-    for (int c = 0; c < H; c += kSlice) store_raw8<T, kVec>(drows + r * H + c, H - c, lane, z);
-    return;
-  }
-  __shared__ float part[kWarps][KF_SORT_MAX_TOP_K];
-  const int64_t t = blockIdx.x;
-  int my_row = -1;
-  float my_w = 1.f;
-  if (lane < K) {
-    my_row = pair_row[t * K + lane];
-    if (my_row >= R) my_row = -1;
-    if (weight) my_w = weight[t * K + lane];
-  }
-  for (int k = 0; k < K; ++k) {
-    const int row = __shfl_sync(0xffffffffu, my_row, k);
-    const float w = __shfl_sync(0xffffffffu, my_w, k);
-    float dot = 0.f;
-    if (row >= 0) {
-      for (int c = warp * kSlice; c < H; c += kWarps * kSlice) {
-        float g[8];
-        to_floats(load_raw8<T, kVec>(dout + t * H + c, H - c, lane), g);
-        if (dweight) {
-          float v[8];
-          to_floats(load_raw8<T, kVec>(rows + static_cast<int64_t>(row) * stride + c, H - c, lane), v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dot = fmaf(g[j], v[j], dot);
+      for (int j = 0; j < kStep; ++j) {
+        ti[j] = i;
+        tc[j] = sl * kSlice;
+        if (u + j * kPlaceWarps < units)
+          v[j] = load_raw8<T, kVec>(x + static_cast<int64_t>(r0 + i) * a.stride + tc[j], a.H - tc[j], lane);
+        sl += kPlaceWarps;
+        while (sl >= slices) {
+          sl -= slices;
+          ++i;
         }
-        if (drows) {
+      }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) g[j] *= w;
-          store_raw8<T, kVec>(drows + static_cast<int64_t>(row) * H + c, H - c, lane, from_floats<T>(g));
+      for (int j = 0; j < kStep; ++j) {
+        if (u + j * kPlaceWarps >= units) break;
+        for (int k = 0; k < a.K; ++k) {
+          const int row = srow[ti[j] * a.K + k];
+          if (row >= 0) store_raw8<T, kVec>(rows + static_cast<int64_t>(row) * a.H + tc[j], a.H - tc[j], lane, v[j]);
         }
       }
     }
+  }
+
+  __syncthreads();   // zero_upto (a block without tokens)
+  const int zeros = zero_upto[kEG];
+  // kCopy: a block per row without a pair; else a thread per row
+  for (int q = kCopy ? blockIdx.x : blockIdx.x * kPlaceThreads + tid; q < zeros; q += kCopy ? G : G * kPlaceThreads) {
+    int lo = 0, hi = kEG;   // the first entry whose zero_upto is above q
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (zero_upto[mid] > q) hi = mid; else lo = mid + 1;
+    }
+    const int64_t row = zero_first[lo] + q - (lo > 0 ? zero_upto[lo - 1] : 0);
+    if (kCopy) {
+      const Raw8<T> z = {};
+      for (int s = warp; s < slices; s += kPlaceWarps)
+        store_raw8<T, kVec>(rows + row * a.H + s * kSlice, a.H - s * kSlice, lane, z);
+      if (tid == 0) a.row_pair[row] = -1;
+    } else {
+      a.row_pair[row] = -1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- scatter --
+
+// A token's rows and weights, lane k holding pair k's (row -1 and weight 0 without one).
+struct PairLane {
+  int row;
+  float w;
+};
+__device__ __forceinline__ PairLane load_pair(const int32_t* __restrict__ pair_row, const float* __restrict__ weight,
+                                              int64_t t, int K, int R, int lane) {
+  PairLane p{-1, 0.f};
+  if (lane < K) {
+    p.row = pair_row[t * K + lane];
+    if (p.row >= R) p.row = -1;
+    if (p.row >= 0) p.w = weight ? weight[t * K + lane] : 1.f;
+  }
+  return p;
+}
+
+// rows[pair_row[t, k]] = x[t] (times weight[t, k] with kWeighted), zeros in the rows
+// of no pair.  A block holds a token's row across its warps, two slices each, reads
+// it once and stores it K times; one block per token and not a loop over tokens:
+// blocks that start in token order keep each expert's segment filling in address
+// order, which the memory wants (4096 tokens, K = 8, 14336-byte rows: 86 us
+// against 99 us for blocks that stay and loop).
+template <typename T, bool kVec, bool kWeighted>
+__global__ void __launch_bounds__(kScatterWarps * 32) scatter_rows_kernel(
+    const T* __restrict__ x, int64_t stride, const int32_t* __restrict__ pair_row, const int32_t* __restrict__ row_pair,
+    const float* __restrict__ weight, int T_, int K, int H, int R, int warps, int tokens, unsigned token_blocks,
+    T* __restrict__ rows) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x >= token_blocks) {
+    grid_dep_wait();
+    zero_rows<T, kVec>(row_pair, static_cast<int64_t>(T_) * K, blockIdx.x - token_blocks, gridDim.x - token_blocks, R, H,
+                       rows);
+    return;
+  }
+  const int sub = warp / warps;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + sub;
+  const bool live = t < T_;
+  bool first = true;
+  PairLane mine{-1, 0.f};
+  for (int c = (warp - sub * warps) * kSlice; c < H; c += 2 * warps * kSlice) {
+    const int c2 = c + warps * kSlice;
+    const Raw8<T> v0 = load_raw8<T, kVec>(x + (live ? t * stride : 0) + c, live ? H - c : 0, lane);
+    const Raw8<T> v1 = load_raw8<T, kVec>(x + (live ? t * stride : 0) + c2, live ? H - c2 : 0, lane);
+    if (first) {   // the order may still be on its way; x is not
+      grid_dep_wait();
+      if (live) mine = load_pair(pair_row, weight, t, K, R, lane);
+      first = false;
+    }
+    for (int k = 0; k < K; ++k) {
+      const int row = __shfl_sync(0xffffffffu, mine.row, k);
+      if (row < 0) continue;
+      T* dst = rows + static_cast<int64_t>(row) * H;
+      if constexpr (kWeighted) {
+        const float w = __shfl_sync(0xffffffffu, mine.w, k);
+        float f[8], g[8];
+        to_floats(v0, f);
+        to_floats(v1, g);
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    if (lane == 0) part[warp][k] = dot;
+        for (int j = 0; j < 8; ++j) {
+          f[j] *= w;
+          g[j] *= w;
+        }
+        store_raw8<T, kVec>(dst + c, H - c, lane, from_floats<T>(f));
+        store_raw8<T, kVec>(dst + c2, H - c2, lane, from_floats<T>(g));
+      } else {
+        store_raw8<T, kVec>(dst + c, H - c, lane, v0);
+        store_raw8<T, kVec>(dst + c2, H - c2, lane, v1);
+      }
+    }
+  }
+}
+
+template <typename T, bool kVec, bool kWeighted>
+cudaError_t launch_scatter(const void* x, int64_t stride, const int32_t* pair_row, const int32_t* row_pair,
+                           const float* weight, int T_, int K, int H, int R, void* rows, bool chained, cudaStream_t s) {
+  const ScatterPlan p = plan_scatter((H + kSlice - 1) / kSlice);
+  const int nwarp = p.warps * p.tokens;
+  const unsigned token_blocks = (static_cast<unsigned>(T_) + p.tokens - 1) / p.tokens;
+  const dim3 grid(token_blocks + zero_blocks_for(R)), block(nwarp * 32);
+  if (grid.x == 0) return cudaSuccess;
+  auto* kernel = scatter_rows_kernel<T, kVec, kWeighted>;
+  if (chained)
+    return launch_chained(kernel, grid, block, 0, s, static_cast<const T*>(x), stride, pair_row, row_pair, weight, T_, K,
+                          H, R, p.warps, p.tokens, token_blocks, static_cast<T*>(rows));
+  kernel<<<grid, block, 0, s>>>(static_cast<const T*>(x), stride, pair_row, row_pair, weight, T_, K, H, R, p.warps,
+                                p.tokens, token_blocks, static_cast<T*>(rows));
+  return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------- combine --
+
+
+// ---- the pipelined form, for 16-byte rows ----
+//
+// Both directions read every pair's row once (K times the output) and are bound by
+// memory.  A block of up to 14 warps (7 for fp32) works on one token at a time, each
+// warp on every W-th slice; a step's loads -- up to eight rows, and the output's
+// gradient in the backward pass -- go by cp.async straight to shared memory, into
+// the lane's own 16-byte slots, while the step before is summed: no barrier, no
+// registers held by loads in flight.  Blocks stay and loop over the tokens, as many
+// as fit the SMs.  Measured (4096 tokens, K = 8, 14336-byte rows of bf16): forward
+// 84 us = 6.3 TB/s against 99 us with the loads in registers, backward 160 us against
+// 191 us; in the backward pass one wide block per SM beats several narrow ones (172 us
+// with six blocks of four warps), as its stores cover longer runs of each row.
+constexpr int kStages = 2;
+template <typename T>
+constexpr int kPipeWarps = sizeof(T) == 4 ? 7 : 14;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// This lane's eight elements of a slot row (512 bytes per 16-byte access of a warp).
+template <typename T>
+__device__ __forceinline__ Raw8<T> slot_load(const uint4* slot) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    const uint4 q = slot[i * 32];
+    r.x[4 * i] = q.x;
+    r.x[4 * i + 1] = q.y;
+    r.x[4 * i + 2] = q.z;
+    r.x[4 * i + 3] = q.w;
+  }
+  return r;
+}
+
+struct CombineArgs {
+  const void* rows;
+  const void* dout;        // backward
+  const int32_t* pair_row;
+  const int32_t* row_pair; // backward with drows
+  const float* weight;
+  void* out;               // forward: output; backward: drows or null
+  float* dweight;
+  int64_t stride;
+  int T, K, H, R;
+};
+
+// kRows rows per step, kBatches steps per slice (K <= kRows * kBatches).
+template <typename T, int kRows, int kBatches, bool kBackward>
+__global__ void __launch_bounds__(kPipeWarps<T> * 32) combine_pipe_kernel(const CombineArgs a) {
+  constexpr int kHalves = sizeof(T) / 2;                     // 16-byte accesses per lane and row
+  constexpr int kSlots = kRows + (kBackward ? 1 : 0);        // the last one: the output's gradient
+  extern __shared__ __align__(16) uint4 pipe_smem[];
+  __shared__ float part[2][kPipeWarps<T>][kRows * kBatches];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+  const uint4* mine = pipe_smem + static_cast<size_t>(warp) * kStages * kSlots * kHalves * 32 + lane;
+  const uint32_t mine_s = smem_u32(mine);
+  const T* rows = static_cast<const T*>(a.rows);
+  const T* dout = static_cast<const T*>(a.dout);
+  const int slices = (a.H + kSlice - 1) / kSlice;
+
+  // the stream of steps to issue, kStages - 1 ahead of the ones summed: token, slice, batch
+  int it = blockIdx.x, is = warp, ib = 0;
+  auto row_of = [&](int t) {
+    int r = -1;
+    if (t < a.T && lane < a.K) r = a.pair_row[static_cast<int64_t>(t) * a.K + lane];
+    return r < a.R ? r : -1;
+  };
+  int row_now = row_of(it), row_next = row_of(it + gridDim.x < static_cast<unsigned>(a.T) ? it + gridDim.x : a.T);
+  auto issue = [&](int stage) {
+    if (it < a.T) {
+      const int c = is * kSlice;
+      const uint32_t dst = mine_s + stage * kSlots * kHalves * 512;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int row = __shfl_sync(0xffffffffu, row_now, ib * kRows + j);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const int col = c + vec_col<T>(lane, h);
+          const bool live = row >= 0 && col < a.H;
+          cp_async16(dst + (j * kHalves + h) * 512, rows + (live ? static_cast<int64_t>(row) * a.stride + col : 0), live);
+        }
+      }
+      if (kBackward) {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const int col = c + vec_col<T>(lane, h);
+          const bool live = col < a.H;
+          cp_async16(dst + (kRows * kHalves + h) * 512, dout + (live ? static_cast<int64_t>(it) * a.H + col : 0), live);
+        }
+      }
+      if (++ib == kBatches) {
+        ib = 0;
+        is += W;
+        if (is >= slices) {
+          is = warp;
+          it = it + gridDim.x < static_cast<unsigned>(a.T) ? it + gridDim.x : a.T;
+          row_now = row_next;
+          row_next = row_of(it + gridDim.x < static_cast<unsigned>(a.T) ? it + gridDim.x : a.T);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+  int stage = 0, par = 0;
+  for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+    const PairLane pair = load_pair(a.pair_row, a.weight, t, a.K, a.R, lane);
+    float dot[kBatches][kRows] = {};
+    for (int sl = warp; sl < slices; sl += W) {
+      const int c = sl * kSlice, n = a.H - c;
+      float acc[8] = {};
+#pragma unroll
+      for (int b = 0; b < kBatches; ++b) {
+        issue(stage == 0 ? kStages - 1 : stage - 1);
+        cp_async_wait<kStages - 1>();   // the oldest step's copies, all of this lane's own
+        const uint4* slot = mine + stage * kSlots * kHalves * 32;
+        if (!kBackward) {
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
+            float f[8];
+            to_floats(slot_load<T>(slot + j * kHalves * 32), f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+          }
+        } else {
+          float g[8];
+          to_floats(slot_load<T>(slot + kRows * kHalves * 32), g);
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            const int row = __shfl_sync(0xffffffffu, pair.row, b * kRows + j);
+            const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
+            float f[8];
+            to_floats(slot_load<T>(slot + j * kHalves * 32), f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot[b][j] = fmaf(g[i], f[i], dot[b][j]);
+            if (a.out && row >= 0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = w * g[i];
+              store_raw8<T, true>(static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
+            }
+          }
+        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+      }
+      if (!kBackward)
+        store_raw8<T, true>(static_cast<T*>(a.out) + static_cast<int64_t>(t) * a.H + c, n, lane, from_floats<T>(acc));
+    }
+    if (kBackward) {
+#pragma unroll
+      for (int b = 0; b < kBatches; ++b)
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+          float d = dot[b][j];
+#pragma unroll
+          for (int off = 16; off >= 1; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+          if (lane == 0) part[par][warp][b * kRows + j] = d;
+        }
+      __syncthreads();   // one per token: the next token writes the other half of `part`
+      if (threadIdx.x < a.K) {
+        float sum = 0.f;
+        if (pair.row >= 0)
+          for (int w = 0; w < W; ++w) sum += part[par][w][threadIdx.x];
+        a.dweight[static_cast<int64_t>(t) * a.K + threadIdx.x] = sum;
+      }
+      par ^= 1;
+    }
+  }
+  cp_async_wait<0>();
+  if (kBackward && a.out)
+    zero_rows<T, true>(a.row_pair, static_cast<int64_t>(a.T) * a.K, blockIdx.x, gridDim.x, a.R, a.H, static_cast<T*>(a.out));
+}
+
+template <typename T, int kRows, int kBatches, bool kBackward>
+cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
+  constexpr int kWarpBytes = kStages * (kRows + (kBackward ? 1 : 0)) * kSlice * static_cast<int>(sizeof(T));
+  auto* kernel = combine_pipe_kernel<T, kRows, kBatches, kBackward>;
+  // the warps that share the slices evenly, and blocks for about kPipeWarps warps on each SM
+  const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kPipeWarps<T> - 1) / kPipeWarps<T>;
+  const int warps = (slices + steps - 1) / steps;
+  const int target = kPipeWarps<T> * 8 / kRows, per_sm = std::max(1, (target + warps / 2) / warps);
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kWarpBytes * kPipeWarps<T>);
+  if (e != cudaSuccess) return e;
+  const int grid = std::min(a.T, sms * per_sm);
+  kernel<<<grid, warps * 32, kWarpBytes * warps, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, bool kBackward>
+cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
+  if (a.K <= 4) return launch_pipe<T, 4, 1, kBackward>(a, sms, s);
+  if (a.K <= 8) return launch_pipe<T, 8, 1, kBackward>(a, sms, s);
+  return launch_pipe<T, 8, 2, kBackward>(a, sms, s);
+}
+
+// ---- the plain form, for rows of any alignment ----
+
+constexpr int kRowWarps = 8;
+template <typename T>
+constexpr int kBatch = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight together
+
+// One warp per (token, slice of 256 columns), consecutive warps on consecutive slices.
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const T* __restrict__ rows, int64_t stride, int R,
+                                                                 const int32_t* __restrict__ pair_row,
+                                                                 const float* __restrict__ weight, int T_, int K, int H,
+                                                                 T* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const unsigned slices = (H + kSlice - 1) / kSlice;
+  const unsigned u = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  const int64_t t = u / slices;
+  if (t >= T_) return;
+  const int c = static_cast<int>(u % slices) * kSlice, n = H - c;
+  const PairLane mine = load_pair(pair_row, weight, t, K, R, lane);
+  float acc[8] = {};
+  for (int k0 = 0; k0 < K; k0 += kBatch<T>) {
+    Raw8<T> v[kBatch<T>];
+    float w[kBatch<T>];
+#pragma unroll
+    for (int j = 0; j < kBatch<T>; ++j) {
+      const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);   // lanes past K hold no row
+      w[j] = __shfl_sync(0xffffffffu, mine.w, k0 + j);
+      v[j] = load_raw8<T, false>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * stride + c, row < 0 ? 0 : n, lane);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch<T>; ++j) {
+      float f[8];
+      to_floats(v[j], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+    }
+  }
+  store_raw8<T, false>(out + t * H + c, n, lane, from_floats<T>(acc));
+}
+
+// Blocks [0, T): one per token, its slices shared by the block's warps.  Blocks
+// past T zero the rows without a pair.
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(
+    const T* __restrict__ dout, const T* __restrict__ rows, int64_t stride, int R, const int32_t* __restrict__ pair_row,
+    const int32_t* __restrict__ row_pair, const float* __restrict__ weight, int T_, int K, int H, T* __restrict__ drows,
+    float* __restrict__ dweight) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+  if (blockIdx.x >= T_) {
+    zero_rows<T, false>(row_pair, static_cast<int64_t>(T_) * K, blockIdx.x - T_, gridDim.x - T_, R, H, drows);
+    return;
+  }
+  __shared__ float part[kRowWarps][KF_SORT_MAX_TOP_K];
+  const int64_t t = blockIdx.x;
+  const PairLane mine = load_pair(pair_row, weight, t, K, R, lane);
+  for (int k0 = 0; k0 < K; k0 += kBatch<T>) {
+    float dot[kBatch<T>] = {};
+    for (int c = warp * kSlice; c < H; c += nwarp * kSlice) {
+      const int n = H - c;
+      const Raw8<T> graw = load_raw8<T, false>(dout + t * H + c, n, lane);
+      float g[8];
+      if (dweight) {
+        Raw8<T> v[kBatch<T>];
+#pragma unroll
+        for (int j = 0; j < kBatch<T>; ++j) {
+          const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
+          v[j] = load_raw8<T, false>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * stride + c, row < 0 ? 0 : n, lane);
+        }
+        to_floats(graw, g);
+#pragma unroll
+        for (int j = 0; j < kBatch<T>; ++j) {
+          float f[8];
+          to_floats(v[j], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
+        }
+      } else {
+        to_floats(graw, g);
+      }
+      if (drows) {
+#pragma unroll
+        for (int j = 0; j < kBatch<T>; ++j) {
+          const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
+          const float w = __shfl_sync(0xffffffffu, mine.w, k0 + j);
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = w * g[i];
+          if (row >= 0) store_raw8<T, false>(drows + static_cast<int64_t>(row) * H + c, n, lane, from_floats<T>(f));
+        }
+      }
+    }
+    if (dweight) {
+#pragma unroll
+      for (int j = 0; j < kBatch<T>; ++j) {
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
+        if (lane == 0 && k0 + j < K) part[warp][k0 + j] = dot[j];
+      }
+    }
   }
   if (!dweight) return;
   __syncthreads();
   if (threadIdx.x < K) {
     float s = 0.f;
-    for (int w = 0; w < kWarps; ++w) s += part[w][threadIdx.x];
+    if (mine.row >= 0)   // lane k of warp 0 holds pair k
+      for (int w = 0; w < nwarp; ++w) s += part[w][threadIdx.x];
     dweight[t * K + threadIdx.x] = s;
   }
 }
@@ -226,11 +675,13 @@ bool valid_shape(int32_t T, int32_t K, int64_t H, int32_t dtype) {
   return valid_tokens(T) && K >= 1 && K <= KF_SORT_MAX_TOP_K && H >= 1 && H <= KF_SORT_MAX_WIDTH && valid_dtype(dtype);
 }
 
-// Launch checks shared by the entry points: grids of one block per token or per few rows stay below 2^31.
-int ready() {
-  int sms = 0;
-  return device_ready(&sms);
-}
+// Calls whose rows are at most this many bytes in all are placed and copied in one launch.
+constexpr int64_t kFusedBytes = 8 << 20;
+
+template <typename P>
+using ElemOf = std::remove_const_t<std::remove_pointer_t<P>>;
+
+inline int code(cudaError_t e) { return e == cudaSuccess ? KF_OK : KF_ERR_CUDA; }
 
 }  // namespace
 }  // namespace kf
@@ -242,9 +693,8 @@ extern "C" {
 size_t kf_sort_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t num_experts) {
   if (!valid_tokens(num_tokens) || top_k < 1 || top_k > KF_SORT_MAX_TOP_K || num_experts < 1 || num_experts > kEG)
     return 0;
-  const int64_t n = static_cast<int64_t>(num_tokens) * top_k;
-  const int64_t nchunk = (n + kOrderChunk - 1) / kOrderChunk;
-  return static_cast<size_t>(nchunk > 0 ? nchunk : 1) * num_experts * sizeof(int32_t);
+  const OrderPlan plan = plan_order(num_tokens, top_k);
+  return static_cast<size_t>(plan.nchunk > 0 ? plan.nchunk : 1) * num_experts * sizeof(int32_t);
 }
 
 int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t* topk_idx, int32_t num_tokens,
@@ -262,29 +712,54 @@ int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t
   const size_t need = kf_sort_workspace_bytes(num_tokens, top_k, num_experts);
   if (!workspace) return KF_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < need) return KF_ERR_WORKSPACE_TOO_SMALL;
-  const int rc = ready();
+  int sms = 0;
+  const int rc = device_ready(&sms);
   if (rc != KF_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int n = num_tokens * top_k;
-  const int nchunk = (n + kOrderChunk - 1) / kOrderChunk;
-  int32_t* hist = static_cast<int32_t*>(workspace);
-  if (num_rows && cudaMemsetAsync(row_pair, 0xff, static_cast<size_t>(num_rows) * 4, s) != cudaSuccess) return KF_ERR_CUDA;
-  if (nchunk) order_hist_kernel<<<nchunk, kOrderThreads, 0, s>>>(topk_idx, n, num_experts, expert_offset, hist);
-  order_scan_kernel<<<1, kOrderThreads, 0, s>>>(hist, nchunk, num_experts, row_align, num_rows, counts, starts);
-  if (nchunk)
-    order_place_kernel<<<nchunk, kOrderThreads, 0, s>>>(topk_idx, n, num_experts, expert_offset, hist, num_rows,
-                                                        pair_row, row_pair);
-  if (cudaGetLastError() != cudaSuccess) return KF_ERR_CUDA;
-  if (num_rows == 0) return KF_OK;
+  const OrderPlan plan = plan_order(num_tokens, top_k);
+  PlaceArgs a;
+  a.ids = topk_idx;
+  a.hist = static_cast<const int32_t*>(workspace);
+  a.T = num_tokens;
+  a.K = top_k;
+  a.H = width;
+  a.E = num_experts;
+  a.offset = expert_offset;
+  a.align = row_align;
+  a.R = num_rows;
+  a.chunk_tokens = plan.chunk_tokens;
+  a.nchunk = plan.nchunk;
+  a.stride = x_stride;
+  a.pair_row = pair_row;
+  a.row_pair = row_pair;
+  a.counts = counts;
+  a.starts = starts;
+  if (plan.nchunk) {
+    order_hist_kernel<<<plan.nchunk, kHistThreads, 0, s>>>(topk_idx, num_tokens * top_k, num_experts, expert_offset,
+                                                           plan.chunk_tokens * top_k, static_cast<int32_t*>(workspace));
+    if (cudaGetLastError() != cudaSuccess) return KF_ERR_CUDA;
+  }
+  const int slices = (width + kSlice - 1) / kSlice;
   const bool vec = vec_rows(x, x_stride, width, dtype) && vec_rows(rows, width, width, dtype);
-  return dispatch_rows(dtype, vec, [&](auto t, auto v) {
-           using E = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-           gather_tokens_kernel<E, decltype(v)::value><<<blocks(num_rows, kWarps), kRowThreads, 0, s>>>(
-               static_cast<const E*>(x), x_stride, num_tokens, top_k, width, row_pair, num_rows, static_cast<E*>(rows));
-           return cudaGetLastError();
-         }) == cudaSuccess
-             ? KF_OK
-             : KF_ERR_CUDA;
+  const bool fused = static_cast<int64_t>(num_rows) * width * static_cast<int64_t>(elem_bytes(dtype)) <= kFusedBytes;
+  // a block per SM; fewer where there is less than a token, or a step of every warp's zeroing, for each
+  const int64_t work = std::max<int64_t>(num_tokens, static_cast<int64_t>(num_rows) * slices / kPlaceWarps);
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, work)));
+  return code(dispatch_rows(dtype, vec, [&](auto t, auto v) {
+    using E = ElemOf<decltype(t)>;
+    constexpr bool kVec = decltype(v)::value;
+    auto* kernel = fused ? place_tokens_kernel<E, kVec, true> : place_tokens_kernel<E, kVec, false>;
+    cudaError_t e;
+    if (plan.nchunk) {
+      e = launch_chained(kernel, dim3(grid), dim3(kPlaceThreads), 0, s, a, static_cast<const E*>(x), static_cast<E*>(rows));
+    } else {
+      kernel<<<grid, kPlaceThreads, 0, s>>>(a, static_cast<const E*>(x), static_cast<E*>(rows));
+      e = cudaGetLastError();
+    }
+    if (fused || e != cudaSuccess) return e;
+    return launch_scatter<E, kVec, false>(x, x_stride, pair_row, row_pair, nullptr, num_tokens, top_k, width, num_rows,
+                                          rows, true, s);
+  }));
 }
 
 int kf_combine_tokens(const void* rows, int32_t dtype, int64_t rows_stride, int32_t num_rows, const int32_t* pair_row,
@@ -294,19 +769,27 @@ int kf_combine_tokens(const void* rows, int32_t dtype, int64_t rows_stride, int3
     return KF_ERR_INVALID_ARGUMENT;
   if (num_tokens == 0) return KF_OK;
   if (!pair_row || !output || (num_rows > 0 && !rows)) return KF_ERR_INVALID_ARGUMENT;
-  const int rc = ready();
-  if (rc != KF_OK) return rc;
-  const bool vec = vec_rows(rows, rows_stride, width, dtype) && vec_rows(output, width, width, dtype);
   const int64_t units = static_cast<int64_t>(num_tokens) * ((width + kSlice - 1) / kSlice);
-  return dispatch_rows(dtype, vec, [&](auto t, auto v) {
-           using E = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-           combine_kernel<E, decltype(v)::value><<<blocks(units, kWarps), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-               static_cast<const E*>(rows), rows_stride, num_rows, pair_row, topk_weight, num_tokens, top_k, width,
-               static_cast<E*>(output));
-           return cudaGetLastError();
-         }) == cudaSuccess
-             ? KF_OK
-             : KF_ERR_CUDA;
+  if (units > 0xffffffffll - kRowWarps) return KF_ERR_INVALID_ARGUMENT;   // rows of terabytes
+  int sms = 0;
+  const int rc = device_ready(&sms);
+  if (rc != KF_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (num_rows == 0)   // no pair has a row
+    return code(cudaMemsetAsync(output, 0, static_cast<size_t>(num_tokens) * width * elem_bytes(dtype), s));
+  const bool vec = vec_rows(rows, rows_stride, width, dtype) && vec_rows(output, width, width, dtype);
+  return code(dispatch_rows(dtype, vec, [&](auto t, auto v) {
+    using E = ElemOf<decltype(t)>;
+    if constexpr (decltype(v)::value) {
+      return launch_pipe<E, false>(CombineArgs{rows, nullptr, pair_row, nullptr, topk_weight, output, nullptr, rows_stride,
+                                               num_tokens, top_k, width, num_rows}, sms, s);
+    } else {
+      combine_kernel<E><<<blocks(units, kRowWarps), kRowWarps * 32, 0, s>>>(
+          static_cast<const E*>(rows), rows_stride, num_rows, pair_row, topk_weight, num_tokens, top_k, width,
+          static_cast<E*>(output));
+      return cudaGetLastError();
+    }
+  }));
 }
 
 int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype, int64_t rows_stride, int32_t num_rows,
@@ -317,21 +800,37 @@ int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype
   if (num_tokens > 0 && (!grad_output || !pair_row)) return KF_ERR_INVALID_ARGUMENT;
   if (grad_weight && num_rows > 0 && !rows) return KF_ERR_INVALID_ARGUMENT;
   if (grad_rows && num_rows > 0 && !row_pair) return KF_ERR_INVALID_ARGUMENT;
-  const int rc = ready();
+  if (num_rows == 0) grad_rows = nullptr;
+  if (num_tokens == 0) grad_weight = nullptr;
+  if (!grad_weight && !grad_rows) return KF_OK;
+  int sms = 0;
+  const int rc = device_ready(&sms);
   if (rc != KF_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (num_rows == 0)
+    return code(cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(num_tokens) * top_k * sizeof(float), s));
   const bool vec = vec_rows(grad_output, width, width, dtype) && (!grad_weight || vec_rows(rows, rows_stride, width, dtype)) &&
                    (!grad_rows || vec_rows(grad_rows, width, width, dtype));
-  const unsigned grid = num_tokens + (grad_rows ? blocks(num_rows, kWarps) : 0u);
-  if (grid == 0) return KF_OK;
-  return dispatch_rows(dtype, vec, [&](auto t, auto v) {
-           using E = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-           combine_backward_kernel<E, decltype(v)::value><<<grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-               static_cast<const E*>(grad_output), static_cast<const E*>(rows), rows_stride, num_rows, pair_row, row_pair,
-               topk_weight, num_tokens, top_k, width, static_cast<E*>(grad_rows), grad_weight);
-           return cudaGetLastError();
-         }) == cudaSuccess
-             ? KF_OK
-             : KF_ERR_CUDA;
+  return code(dispatch_rows(dtype, vec, [&](auto t, auto v) {
+    using E = ElemOf<decltype(t)>;
+    constexpr bool kVec = decltype(v)::value;
+    if (!grad_weight)   // the rows are not read: scatter the weighted gradient
+      return launch_scatter<E, kVec, true>(grad_output, width, pair_row, row_pair, topk_weight, num_tokens, top_k, width,
+                                           num_rows, grad_rows, false, s);
+    if constexpr (kVec) {
+      return launch_pipe<E, true>(CombineArgs{rows, grad_output, pair_row, row_pair, topk_weight, grad_rows, grad_weight,
+                                              rows_stride, num_tokens, top_k, width, num_rows}, sms, s);
+    } else {
+      // as many warps as share the slices evenly, kRowWarps at most
+      const int slices = (width + kSlice - 1) / kSlice, steps = (slices + kRowWarps - 1) / kRowWarps;
+      const int warps = (slices + steps - 1) / steps;
+      const unsigned grid = num_tokens + (grad_rows ? zero_blocks_for(num_rows) : 0u);
+      combine_backward_kernel<E><<<grid, warps * 32, 0, s>>>(
+          static_cast<const E*>(grad_output), static_cast<const E*>(rows), rows_stride, num_rows, pair_row, row_pair,
+          topk_weight, num_tokens, top_k, width, static_cast<E*>(grad_rows), grad_weight);
+      return cudaGetLastError();
+    }
+  }));
 }
 
 }  // extern "C"

@@ -150,6 +150,7 @@ struct SortFn : public torch::autograd::Function<SortFn> {
   static variable_list forward(AutogradContext* ctx, const Variable& x, const Variable& ids, int64_t experts,
                                int64_t offset, int64_t align, int64_t rows) {
     variable_list out = sort_forward(x, ids, SortArgs{experts, offset, align, rows});
+    ctx->set_materialize_grads(false);   // no zeros in place of the integer outputs' gradients
     ctx->mark_non_differentiable({out[1], out[2], out[3], out[4]});
     ctx->save_for_backward({out[1]});
     return out;
@@ -287,6 +288,7 @@ variable_list route_forward(const Tensor& logits, const Tensor& bias, double rsf
 struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, const Variable& logits, const Variable& bias, double rsf) {
     variable_list out = route_forward(logits, bias, rsf);
+    ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[0]});
     ctx->save_for_backward({logits, out[0]});
     ctx->saved_data["rsf"] = rsf;
@@ -348,37 +350,44 @@ Tensor restore8(const Tensor& codes_in, const Tensor& exps_in, at::ScalarType dt
   const at::Device dev = codes.device();
   c10::cuda::CUDAGuard guard(dev);
   int64_t out_rows = codes.size(0), K = 0;
-  Tensor map;
+  Tensor pairs, map;
   if (row_pair.has_value()) {
     const Order o = expect_order(*pair_row, *row_pair, dev);
     TORCH_CHECK(o.pair_row.size(0) == codes.size(0), "kept has ", codes.size(0), " rows, the order ",
                 o.pair_row.size(0), " tokens");
+    pairs = o.pair_row;
     map = o.row_pair;
     out_rows = map.size(0);
     K = o.pair_row.size(1);
   }
   Tensor out = at::empty({out_rows, codes.size(1)}, codes.options().dtype(dtype));
   check_rc(kf_restore8(ptr(codes), ptr(exps), dtype_of(out, "kept.dtype"), static_cast<int32_t>(codes.size(0)),
-                       static_cast<int32_t>(codes.size(1)), map.defined() ? map.const_data_ptr<int32_t>() : nullptr,
+                       static_cast<int32_t>(codes.size(1)), pairs.defined() ? pairs.const_data_ptr<int32_t>() : nullptr,
+                       map.defined() ? map.const_data_ptr<int32_t>() : nullptr,
                        static_cast<int32_t>(K), static_cast<int32_t>(out_rows), ptr(out), stream_of(dev)),
            "kf_restore8");
   return out;
 }
 
-std::tuple<Tensor, Tensor, Tensor> swiglu_pack8(const Tensor& h_in) {
+std::tuple<Tensor, Tensor, Tensor> swiglu_forward(const Tensor& h_in, bool keep) {
   const Tensor h = expect_rows(h_in.detach(), "h");
   TORCH_CHECK(h.size(1) % 2 == 0, "h must be [R, 2 I] = [up | gate], got shape ", h.sizes());
   check_num_rows(h.size(0), "number of rows");
   const int64_t R = h.size(0), I = h.size(1) / 2;
   c10::cuda::CUDAGuard guard(h.device());
   Tensor act = at::empty({R, I}, h.options());
-  Tensor codes = at::empty({R, 2 * I}, h.options().dtype(at::kFloat8_e4m3fn));
-  Tensor exps = at::empty({R, 2 * blocks_of(I)}, h.options().dtype(at::kByte));
+  Tensor codes, exps;
+  if (keep) {
+    codes = at::empty({R, 2 * I}, h.options().dtype(at::kFloat8_e4m3fn));
+    exps = at::empty({R, 2 * blocks_of(I)}, h.options().dtype(at::kByte));
+  }
   check_rc(kf_swiglu_pack8(ptr(h), dtype_of(h, "h"), h.stride(0), static_cast<int32_t>(R), static_cast<int32_t>(I),
                            ptr(act), ptr(codes), ptr(exps), stream_of(h.device())),
            "kf_swiglu_pack8");
   return {act, codes, exps};
 }
+
+std::tuple<Tensor, Tensor, Tensor> swiglu_pack8(const Tensor& h) { return swiglu_forward(h, true); }
 
 std::tuple<Tensor, Tensor> swiglu_backward8(const Tensor& codes_in, const Tensor& exps_in, const Tensor& grad_act,
                                             bool need_act) {
@@ -413,7 +422,7 @@ struct SwigluFn : public torch::autograd::Function<SwigluFn> {
 
 Tensor swiglu(const Tensor& h) {
   if (wants_grad(h)) return SwigluFn::apply(h);
-  return std::get<0>(swiglu_pack8(h));
+  return std::get<0>(swiglu_forward(h, false));
 }
 
 }  // namespace

@@ -151,18 +151,18 @@ def test_combine_backward_refuses_bad_arguments_before_device_work(bad):
 def test_the_8_bit_entry_points_refuse_bad_arguments_before_device_work():
     lib = B.library()
     lib.kf_pack8.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp]
-    lib.kf_restore8.argtypes = [vp, vp, i32, i32, i32, vp, i32, i32, vp, vp]
+    lib.kf_restore8.argtypes = [vp, vp, i32, i32, i32, vp, vp, i32, i32, vp, vp]
     lib.kf_swiglu_pack8.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp]
     lib.kf_swiglu_backward8.argtypes = [vp, vp, vp, i32, i64, i32, i32, vp, vp, vp]
     ok = (SOME, 0, 64, 4, 64, SOME, SOME, NULL)
     for i, v in ((0, NULL), (1, 3), (2, -1), (3, -1), (4, 0), (4, (1 << 20) + 1), (5, NULL), (6, NULL)):
         assert lib.kf_pack8(*(v if j == i else a for j, a in enumerate(ok))) == 1
-    ok = (SOME, SOME, 0, 4, 64, SOME, 2, 8, SOME, NULL)
-    for i, v in ((0, NULL), (1, NULL), (2, 9), (3, -1), (4, 0), (6, 0), (6, 17), (7, -1), (8, NULL)):
+    ok = (SOME, SOME, 0, 4, 64, SOME, SOME, 2, 8, SOME, NULL)
+    for i, v in ((0, NULL), (1, NULL), (2, 9), (3, -1), (3, (1 << 24) + 1), (4, 0), (5, NULL), (7, 0), (7, 17), (8, -1), (9, NULL)):
         assert lib.kf_restore8(*(v if j == i else a for j, a in enumerate(ok))) == 1
-    assert lib.kf_restore8(SOME, SOME, 0, 4, 64, NULL, 0, 5, SOME, NULL) == 1   # without an order the rows stay as many
+    assert lib.kf_restore8(SOME, SOME, 0, 4, 64, NULL, NULL, 0, 5, SOME, NULL) == 1   # without an order the rows stay as many
     ok = (SOME, 0, 128, 4, 64, SOME, SOME, SOME, NULL)
-    for i, v in ((0, NULL), (1, -1), (2, -1), (3, -1), (4, 0), (5, NULL)):
+    for i, v in ((0, NULL), (1, -1), (2, -1), (3, -1), (4, 0), (5, NULL), (6, NULL), (7, NULL)):
         assert lib.kf_swiglu_pack8(*(v if j == i else a for j, a in enumerate(ok))) == 1
     ok = (SOME, SOME, SOME, 0, 64, 4, 64, SOME, SOME, NULL)
     for i, v in ((0, NULL), (1, NULL), (2, NULL), (3, 3), (4, -1), (5, -1), (6, 0), (7, NULL)):
