@@ -4,8 +4,10 @@
 // 16-byte aligned rows and a width that is a multiple of 8, a lane's accesses are 16
 // bytes: lane l holds columns 8l .. 8l+7 of 16-bit types, and 4l .. 4l+3 and
 // 128 + 4l .. 128 + 4l+3 of fp32, so that each access of a warp is one run of 512
-// bytes.  Otherwise lane l holds columns l + 32 j, one element per access.
-// Arithmetic is fp32 whatever the element type.
+// bytes.  Otherwise accesses are 4 bytes: lane l holds columns l + 32 j of fp32, and
+// the pairs 2l + 64 j, 2l + 64 j + 1 of 16-bit types, which a row that starts between
+// two 4-byte words takes from its neighbours' words by shuffles.  Nothing outside
+// the row is read or written.  Arithmetic is fp32 whatever the element type.
 #pragma once
 
 #include <cstdint>
@@ -81,17 +83,43 @@ __device__ __forceinline__ Raw8<T> load_raw8(const T* __restrict__ slice, int n,
       r.x[4 * i + 2] = v.z;
       r.x[4 * i + 3] = v.w;
     }
-  } else if (sizeof(T) == 4) {
+  } else if constexpr (sizeof(T) == 4) {
     const uint32_t* p = reinterpret_cast<const uint32_t*>(slice);
+    if (n >= kSlice) {   // without conditions the loads go out together
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r.x[j % (sizeof(T) * 2)] = lane + 32 * j < n ? __ldg(p + lane + 32 * j) : 0u;
+      for (int j = 0; j < 8; ++j) r.x[j] = __ldg(p + lane + 32 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r.x[j] = lane + 32 * j < n ? __ldg(p + lane + 32 * j) : 0u;
+    }
   } else {
     const unsigned short* p = reinterpret_cast<const unsigned short*>(slice);
+    const bool even = (reinterpret_cast<uintptr_t>(slice) & 3u) == 0;
+    if (n >= kSlice && even) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = lane + 64 * j < n ? __ldg(p + lane + 64 * j) : 0u;
-      const uint32_t hi = lane + 64 * j + 32 < n ? __ldg(p + lane + 64 * j + 32) : 0u;
-      r.x[j] = lo | (hi << 16);
+      for (int j = 0; j < 4; ++j) r.x[j] = __ldg(reinterpret_cast<const uint32_t*>(p) + lane + 32 * j);
+    } else if (n >= kSlice) {
+      // word q holds elements 2q - 1 and 2q; of words 0 and 128 only one element is the slice's
+      uint32_t w[4], last = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int q = lane + 32 * j;
+        w[j] = q == 0 ? static_cast<uint32_t>(__ldg(p)) << 16 : __ldg(reinterpret_cast<const uint32_t*>(p - 1) + q);
+      }
+      if (lane == 31) last = __ldg(p + kSlice - 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t up = __shfl_sync(0xffffffffu, w[j], (lane + 1) & 31);                 // word q + 1 of lanes 0..30
+        const uint32_t wrap = j < 3 ? __shfl_sync(0xffffffffu, w[j < 3 ? j + 1 : 3], 0) : last;   // and of lane 31
+        r.x[j] = __funnelshift_r(w[j], lane == 31 ? wrap : up, 16);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = 2 * lane + 64 * j;
+        const uint32_t lo = c < n ? __ldg(p + c) : 0u, hi = c + 1 < n ? __ldg(p + c + 1) : 0u;
+        r.x[j] = lo | (hi << 16);
+      }
     }
   }
   return r;
@@ -105,19 +133,44 @@ __device__ __forceinline__ void store_raw8(T* __restrict__ slice, int n, int lan
       if (vec_col<T>(lane, i) < n)
         *reinterpret_cast<uint4*>(slice + vec_col<T>(lane, i)) =
             make_uint4(r.x[4 * i], r.x[4 * i + 1], r.x[4 * i + 2], r.x[4 * i + 3]);
-  } else if (sizeof(T) == 4) {
+  } else if constexpr (sizeof(T) == 4) {
     uint32_t* p = reinterpret_cast<uint32_t*>(slice);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (lane + 32 * j < n) p[lane + 32 * j] = r.x[j % (sizeof(T) * 2)];
+      if (lane + 32 * j < n) p[lane + 32 * j] = r.x[j];
   } else {
     unsigned short* p = reinterpret_cast<unsigned short*>(slice);
+    const bool even = (reinterpret_cast<uintptr_t>(slice) & 3u) == 0;
+    if (n >= kSlice && even) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (lane + 64 * j < n) p[lane + 64 * j] = static_cast<unsigned short>(r.x[j] & 0xffffu);
-      if (lane + 64 * j + 32 < n) p[lane + 64 * j + 32] = static_cast<unsigned short>(r.x[j] >> 16);
+      for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(p)[lane + 32 * j] = r.x[j];
+    } else if (n >= kSlice) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t down = __shfl_sync(0xffffffffu, r.x[j], (lane + 31) & 31);                 // pair q - 1 of lanes 1..31
+        const uint32_t wrap = __shfl_sync(0xffffffffu, r.x[j > 0 ? j - 1 : 0], 31);               // and of lane 0
+        const uint32_t w = __funnelshift_r(lane == 0 ? wrap : down, r.x[j], 16);
+        if (j == 0 && lane == 0)
+          p[0] = static_cast<unsigned short>(r.x[0] & 0xffffu);
+        else
+          reinterpret_cast<uint32_t*>(p - 1)[lane + 32 * j] = w;
+      }
+      if (lane == 31) p[kSlice - 1] = static_cast<unsigned short>(r.x[3] >> 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = 2 * lane + 64 * j;
+        if (c < n) p[c] = static_cast<unsigned short>(r.x[j] & 0xffffu);
+        if (c + 1 < n) p[c + 1] = static_cast<unsigned short>(r.x[j] >> 16);
+      }
     }
   }
+}
+
+// Column of element j of a lane in the form without 16-byte accesses.
+template <typename T>
+__device__ __forceinline__ int word_col(int lane, int j) {
+  return sizeof(T) == 4 ? lane + 32 * j : 2 * lane + 64 * (j >> 1) + (j & 1);
 }
 
 __device__ __forceinline__ void to_floats(const Raw8<float>& r, float (&v)[8]) {

@@ -146,7 +146,8 @@ __device__ __forceinline__ void store_codes(uint8_t* __restrict__ slice, int n, 
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (lane + 32 * j < n) slice[lane + 32 * j] = static_cast<uint8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+      if (word_col<T>(lane, j) < n)
+        slice[word_col<T>(lane, j)] = static_cast<uint8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
   }
 }
 
@@ -161,7 +162,8 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* __restrict__ slice, i
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (lane + 32 * j < n) (j < 4 ? c.x : c.y) |= static_cast<uint32_t>(__ldg(slice + lane + 32 * j)) << (8 * (j & 3));
+      if (word_col<T>(lane, j) < n)
+        (j < 4 ? c.x : c.y) |= static_cast<uint32_t>(__ldg(slice + word_col<T>(lane, j))) << (8 * (j & 3));
   }
   return c;
 }
@@ -215,28 +217,26 @@ __device__ __forceinline__ Unit unit_of(int slices) {
   return Unit{u / groups, static_cast<int>(u % groups) * kGroup};
 }
 
-// Slices per warp whose loads are in flight together.
-constexpr int kPackGroup = 4;
-constexpr int kRestoreGroup = 4;
-template <typename T>
-constexpr int kSwigluGroup = sizeof(T) == 4 ? 1 : 2;
+// Slices per warp whose loads are in flight together: two, where that leaves at
+// most an eighth of the warps half empty, else one.
+inline bool pairs_of_slices(int slices) { return slices % 2 == 0 || slices >= 7; }
 
-template <typename T, bool kVec>
+template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t stride, int R, int W,
                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   const int lane = threadIdx.x & 31;
   const int slices = (W + kSlice - 1) / kSlice, nb = (W + kBlk - 1) / kBlk;
-  const Unit u = unit_of<kPackGroup>(slices);
+  const Unit u = unit_of<kGroup>(slices);
   if (u.row >= R) return;
   const T* src = x + u.row * stride;
-  Raw8<T> raw[kPackGroup];
+  Raw8<T> raw[kGroup];
 #pragma unroll
-  for (int j = 0; j < kPackGroup; ++j) {
+  for (int j = 0; j < kGroup; ++j) {
     const int c = (u.slice + j) * kSlice;
     raw[j] = load_raw8<T, kVec>(src + c, W - c, lane);   // past the width: nothing is read
   }
 #pragma unroll
-  for (int j = 0; j < kPackGroup; ++j) {
+  for (int j = 0; j < kGroup; ++j) {
     const int c = (u.slice + j) * kSlice, n = W - c;
     if (n <= 0) break;
     float v[8];
@@ -259,24 +259,24 @@ __device__ __forceinline__ Raw8<T> restored(uint2 codes, const float (&s)[2]) {
 }
 
 // Rows as they were.
-template <typename T, bool kVec>
+template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __restrict__ codes,
                                                             const uint8_t* __restrict__ exps, int R, int W,
                                                             T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   const int slices = (W + kSlice - 1) / kSlice, nb = (W + kBlk - 1) / kBlk;
-  const Unit u = unit_of<kRestoreGroup>(slices);
+  const Unit u = unit_of<kGroup>(slices);
   if (u.row >= R) return;
-  uint2 q[kRestoreGroup];
-  float s[kRestoreGroup][2];
+  uint2 q[kGroup];
+  float s[kGroup][2];
 #pragma unroll
-  for (int j = 0; j < kRestoreGroup; ++j) {
+  for (int j = 0; j < kGroup; ++j) {
     const int c = (u.slice + j) * kSlice;
     q[j] = load_codes<T, kVec>(codes + u.row * W + c, W - c, lane);
     load_scales<T, kVec>(exps + u.row * nb + c / kBlk, W - c, lane, s[j]);
   }
 #pragma unroll
-  for (int j = 0; j < kRestoreGroup; ++j) {
+  for (int j = 0; j < kGroup; ++j) {
     const int c = (u.slice + j) * kSlice;
     store_raw8<T, kVec>(out + u.row * W + c, W - c, lane, restored<T, kVec>(q[j], s[j]));
   }
@@ -328,11 +328,10 @@ __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
 }
 
 // h = [up | gate]: act = up * silu(gate), and h kept in 8 bits (each half's blocks begin at its own column 0).
-template <typename T, bool kVec>
+template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restrict__ h, int64_t stride, int R, int I,
                                                                 T* __restrict__ act, uint8_t* __restrict__ codes,
                                                                 uint8_t* __restrict__ exps) {
-  constexpr int kGroup = kSwigluGroup<T>;
   const int lane = threadIdx.x & 31;
   const int slices = (I + kSlice - 1) / kSlice, nb = (I + kBlk - 1) / kBlk;
   const Unit unit = unit_of<kGroup>(slices);
@@ -355,7 +354,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] = u[j] * (g[j] * sigmoid(g[j]));
     store_raw8<T, kVec>(act + r * I + c, n, lane, from_floats<T>(a));
-    if (!codes) continue;   // the activation alone
+    if (codes == nullptr) continue;   // the activation alone
     uint32_t ku[2], kg[2];
     max_keys(ru[i], ku);
     max_keys(rg[i], kg);
@@ -373,12 +372,11 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
 }
 
 // From the kept values u, g and d = dL/dact: du = d g s, dg = d u s (1 + g (1 - s)), act = u g s, with s = sigmoid(g).
-template <typename T, bool kVec>
+template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ exps,
                                                                     const T* __restrict__ grad, int64_t stride, int R,
                                                                     int I, T* __restrict__ dh, T* __restrict__ act) {
-  constexpr int kGroup = kSwigluGroup<T>;
   const int lane = threadIdx.x & 31;
   const int slices = (I + kSlice - 1) / kSlice, nb = (I + kBlk - 1) / kBlk;
   const Unit unit = unit_of<kGroup>(slices);
@@ -426,21 +424,30 @@ bool valid_rows(int64_t R, int64_t W, int32_t dtype) {
 }
 
 // Blocks of a grid of one warp per (row, group of slices); 0 when they are too many (rows of terabytes).
-unsigned grid_of(int64_t R, int64_t W, int group) {
-  const int64_t slices = (W + kSlice - 1) / kSlice;
+unsigned grid_of(int64_t R, int64_t W) {
+  const int64_t slices = (W + kSlice - 1) / kSlice, group = pairs_of_slices(static_cast<int>(slices)) ? 2 : 1;
   const int64_t units = R * ((slices + group - 1) / group);
   return units <= 0xffffffffll - kWarps ? static_cast<unsigned>((units + kWarps - 1) / kWarps) : 0u;
 }
 
 inline bool aligned(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+template <int N>
+struct IntTag {
+  static constexpr int value = N;
+};
+
+// Calls f(type, access form, group) for rows of `width` columns.
 template <typename F>
-int launch(int32_t dtype, bool vec, F&& f) {
+int launch(int32_t dtype, bool vec, int32_t width, F&& f) {
   int sms = 0;
   const int rc = device_ready(&sms);
   if (rc != KF_OK) return rc;
   return dispatch_rows(dtype, vec, [&](auto t, auto v) {
-           f(t, v);
+           if (pairs_of_slices((width + kSlice - 1) / kSlice))
+             f(t, v, IntTag<2>{});
+           else
+             f(t, v, IntTag<1>{});
            return cudaGetLastError();
          }) == cudaSuccess
              ? KF_OK
@@ -461,12 +468,12 @@ int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, i
              void* exponents, void* stream) {
   if (!valid_rows(num_rows, width, dtype) || x_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, width, kPackGroup);
+  const unsigned grid = grid_of(num_rows, width);
   if (!x || !codes || !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(x, x_stride, width, dtype) && aligned(codes, 8);
-  return launch(dtype, vec, [&](auto t, auto v) {
+  return launch(dtype, vec, width, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
-    pack8_kernel<E, decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+    pack8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const E*>(x), x_stride, num_rows, width, static_cast<uint8_t*>(codes),
         static_cast<uint8_t*>(exponents));
   });
@@ -482,10 +489,10 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
              : out_rows != num_rows)
     return KF_ERR_INVALID_ARGUMENT;
   if (out_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, width, kRestoreGroup);
+  const unsigned grid = grid_of(num_rows, width);
   if (!output || (num_rows > 0 && !grid)) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(output, width, width, dtype) && aligned(codes, 8);
-  return launch(dtype, vec, [&](auto t, auto v) {
+  return launch(dtype, vec, width, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
     const uint8_t* c = static_cast<const uint8_t*>(codes);
     const uint8_t* e = static_cast<const uint8_t*>(exponents);
@@ -497,7 +504,7 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
           c, e, num_rows, width, pair_row, row_pair, top_k, out_rows, p.warps, p.tokens, token_blocks,
           static_cast<E*>(output));
     } else {
-      restore8_kernel<E, decltype(v)::value><<<grid, kThreads, 0, s>>>(c, e, num_rows, width, static_cast<E*>(output));
+      restore8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, s>>>(c, e, num_rows, width, static_cast<E*>(output));
     }
   });
 }
@@ -506,12 +513,12 @@ int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_
                     void* codes, void* exponents, void* stream) {
   if (!valid_rows(num_rows, inter, dtype) || h_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, inter, dtype == KF_DTYPE_F32 ? kSwigluGroup<float> : kSwigluGroup<__half>);
+  const unsigned grid = grid_of(num_rows, inter);
   if (!h || !act || !codes != !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(h, h_stride, inter, dtype) && vec_rows(act, inter, inter, dtype) && aligned(codes, 8);
-  return launch(dtype, vec, [&](auto t, auto v) {
+  return launch(dtype, vec, inter, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
-    swiglu_pack8_kernel<E, decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+    swiglu_pack8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const E*>(h), h_stride, num_rows, inter, static_cast<E*>(act), static_cast<uint8_t*>(codes),
         static_cast<uint8_t*>(exponents));
   });
@@ -521,13 +528,13 @@ int kf_swiglu_backward8(const void* codes, const void* exponents, const void* gr
                         int64_t grad_stride, int32_t num_rows, int32_t inter, void* grad_h, void* act, void* stream) {
   if (!valid_rows(num_rows, inter, dtype) || grad_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
-  const unsigned grid = grid_of(num_rows, inter, dtype == KF_DTYPE_F32 ? kSwigluGroup<float> : kSwigluGroup<__half>);
+  const unsigned grid = grid_of(num_rows, inter);
   if (!codes || !exponents || !grad_act || !grad_h || !grid) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(grad_act, grad_stride, inter, dtype) && vec_rows(grad_h, inter, inter, dtype) &&
                    (!act || vec_rows(act, inter, inter, dtype)) && aligned(codes, 8);
-  return launch(dtype, vec, [&](auto t, auto v) {
+  return launch(dtype, vec, inter, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
-    swiglu_backward8_kernel<E, decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+    swiglu_backward8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(exponents), static_cast<const E*>(grad_act),
         grad_stride, num_rows, inter, static_cast<E*>(grad_h), static_cast<E*>(act));
   });

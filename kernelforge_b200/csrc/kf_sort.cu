@@ -554,12 +554,15 @@ cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
 
 template <typename T, bool kBackward>
 cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
+  if (a.K <= 2) return launch_pipe<T, 2, 1, kBackward>(a, sms, s);
   if (a.K <= 4) return launch_pipe<T, 4, 1, kBackward>(a, sms, s);
   if (a.K <= 8) return launch_pipe<T, 8, 1, kBackward>(a, sms, s);
   return launch_pipe<T, 8, 2, kBackward>(a, sms, s);
 }
 
-// ---- the plain form, for rows of any alignment ----
+// ---- the plain form, for rows of any alignment (and fp32 backward) ----
+
+inline unsigned blocks(int64_t items, int per) { return static_cast<unsigned>((items + per - 1) / per); }
 
 constexpr int kRowWarps = 8;
 template <typename T>
@@ -567,109 +570,116 @@ constexpr int kBatch = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flig
 
 // One warp per (token, slice of 256 columns), consecutive warps on consecutive slices.
 template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const T* __restrict__ rows, int64_t stride, int R,
-                                                                 const int32_t* __restrict__ pair_row,
-                                                                 const float* __restrict__ weight, int T_, int K, int H,
-                                                                 T* __restrict__ out) {
+__global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const CombineArgs a) {
+  const T* rows = static_cast<const T*>(a.rows);
   const int lane = threadIdx.x & 31;
-  const unsigned slices = (H + kSlice - 1) / kSlice;
+  const unsigned slices = (a.H + kSlice - 1) / kSlice;
   const unsigned u = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   const int64_t t = u / slices;
-  if (t >= T_) return;
-  const int c = static_cast<int>(u % slices) * kSlice, n = H - c;
-  const PairLane mine = load_pair(pair_row, weight, t, K, R, lane);
+  if (t >= a.T) return;
+  const int c = static_cast<int>(u % slices) * kSlice, n = a.H - c;
+  const PairLane mine = load_pair(a.pair_row, a.weight, t, a.K, a.R, lane);
   float acc[8] = {};
-  for (int k0 = 0; k0 < K; k0 += kBatch<T>) {
+  for (int k0 = 0; k0 < a.K; k0 += kBatch<T>) {
     Raw8<T> v[kBatch<T>];
-    float w[kBatch<T>];
 #pragma unroll
     for (int j = 0; j < kBatch<T>; ++j) {
       const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);   // lanes past K hold no row
-      w[j] = __shfl_sync(0xffffffffu, mine.w, k0 + j);
-      v[j] = load_raw8<T, false>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * stride + c, row < 0 ? 0 : n, lane);
+      v[j] = load_raw8<T, false>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * a.stride + c, row < 0 ? 0 : n, lane);
     }
 #pragma unroll
     for (int j = 0; j < kBatch<T>; ++j) {
+      const float w = __shfl_sync(0xffffffffu, mine.w, k0 + j);
       float f[8];
       to_floats(v[j], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
     }
   }
-  store_raw8<T, false>(out + t * H + c, n, lane, from_floats<T>(acc));
+  store_raw8<T, false>(static_cast<T*>(a.out) + t * a.H + c, n, lane, from_floats<T>(acc));
 }
 
-// Blocks [0, T): one per token, its slices shared by the block's warps.  Blocks
-// past T zero the rows without a pair.
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(
-    const T* __restrict__ dout, const T* __restrict__ rows, int64_t stride, int R, const int32_t* __restrict__ pair_row,
-    const int32_t* __restrict__ row_pair, const float* __restrict__ weight, int T_, int K, int H, T* __restrict__ drows,
-    float* __restrict__ dweight) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
-  if (blockIdx.x >= T_) {
-    zero_rows<T, false>(row_pair, static_cast<int64_t>(T_) * K, blockIdx.x - T_, gridDim.x - T_, R, H, drows);
+// `warps` warps per token share its slices, `tokens` tokens per block.  Blocks past
+// the tokens zero the rows without a pair.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(const CombineArgs a, int warps, int tokens,
+                                                                          unsigned token_blocks) {
+  const T* rows = static_cast<const T*>(a.rows);
+  const T* dout = static_cast<const T*>(a.dout);
+  T* drows = static_cast<T*>(a.out);
+  if (blockIdx.x >= token_blocks) {
+    zero_rows<T, kVec>(a.row_pair, static_cast<int64_t>(a.T) * a.K, blockIdx.x - token_blocks, gridDim.x - token_blocks,
+                       a.R, a.H, drows);
     return;
   }
   __shared__ float part[kRowWarps][KF_SORT_MAX_TOP_K];
-  const int64_t t = blockIdx.x;
-  const PairLane mine = load_pair(pair_row, weight, t, K, R, lane);
-  for (int k0 = 0; k0 < K; k0 += kBatch<T>) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = warp / warps, w0 = warp - sub * warps;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + sub;
+  const bool live = t < a.T;
+  PairLane mine{-1, 0.f};
+  if (live) mine = load_pair(a.pair_row, a.weight, t, a.K, a.R, lane);
+  for (int k0 = 0; k0 < a.K; k0 += kBatch<T>) {
     float dot[kBatch<T>] = {};
-    for (int c = warp * kSlice; c < H; c += nwarp * kSlice) {
-      const int n = H - c;
-      const Raw8<T> graw = load_raw8<T, false>(dout + t * H + c, n, lane);
-      float g[8];
-      if (dweight) {
-        Raw8<T> v[kBatch<T>];
-#pragma unroll
-        for (int j = 0; j < kBatch<T>; ++j) {
-          const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
-          v[j] = load_raw8<T, false>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * stride + c, row < 0 ? 0 : n, lane);
-        }
-        to_floats(graw, g);
-#pragma unroll
-        for (int j = 0; j < kBatch<T>; ++j) {
-          float f[8];
-          to_floats(v[j], f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
-        }
-      } else {
-        to_floats(graw, g);
-      }
-      if (drows) {
-#pragma unroll
-        for (int j = 0; j < kBatch<T>; ++j) {
-          const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
-          const float w = __shfl_sync(0xffffffffu, mine.w, k0 + j);
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = w * g[i];
-          if (row >= 0) store_raw8<T, false>(drows + static_cast<int64_t>(row) * H + c, n, lane, from_floats<T>(f));
-        }
-      }
-    }
-    if (dweight) {
+    for (int c = w0 * kSlice; live && c < a.H; c += warps * kSlice) {
+      const int n = a.H - c;
+      Raw8<T> v[kBatch<T>];
+      const Raw8<T> graw = load_raw8<T, kVec>(dout + t * a.H + c, n, lane);
 #pragma unroll
       for (int j = 0; j < kBatch<T>; ++j) {
+        const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
+        v[j] = load_raw8<T, kVec>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * a.stride + c, row < 0 ? 0 : n, lane);
+      }
+      float g[8];
+      to_floats(graw, g);
 #pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
-        if (lane == 0 && k0 + j < K) part[warp][k0 + j] = dot[j];
+      for (int j = 0; j < kBatch<T>; ++j) {
+        const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
+        const float w = __shfl_sync(0xffffffffu, mine.w, k0 + j);
+        float f[8];
+        to_floats(v[j], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
+        if (drows && row >= 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = w * g[i];
+          store_raw8<T, kVec>(drows + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
+        }
       }
     }
+#pragma unroll
+    for (int j = 0; j < kBatch<T>; ++j) {
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
+      if (lane == 0 && k0 + j < a.K) part[warp][k0 + j] = dot[j];
+    }
   }
-  if (!dweight) return;
   __syncthreads();
-  if (threadIdx.x < K) {
+  if (live && w0 == 0 && lane < a.K) {
     float s = 0.f;
-    if (mine.row >= 0)   // lane k of warp 0 holds pair k
-      for (int w = 0; w < nwarp; ++w) s += part[w][threadIdx.x];
-    dweight[t * K + threadIdx.x] = s;
+    if (mine.row >= 0)
+      for (int w = 0; w < warps; ++w) s += part[warp + w][lane];
+    a.dweight[t * a.K + lane] = s;
   }
 }
 
-inline unsigned blocks(int64_t items, int per) { return static_cast<unsigned>((items + per - 1) / per); }
+template <typename T>
+cudaError_t launch_combine(const CombineArgs& a, cudaStream_t s) {
+  const int64_t units = static_cast<int64_t>(a.T) * ((a.H + kSlice - 1) / kSlice);
+  combine_kernel<T><<<blocks(units, kRowWarps), kRowWarps * 32, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, bool kVec>
+cudaError_t launch_combine_backward(const CombineArgs& a, cudaStream_t s) {
+  // as many warps as share the slices evenly, kRowWarps at most
+  const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kRowWarps - 1) / kRowWarps;
+  const int warps = (slices + steps - 1) / steps, tokens = kRowWarps / warps;
+  const unsigned token_blocks = blocks(a.T, tokens);
+  const unsigned grid = token_blocks + (a.out ? zero_blocks_for(a.R) : 0u);
+  combine_backward_kernel<T, kVec><<<grid, warps * tokens * 32, 0, s>>>(a, warps, tokens, token_blocks);
+  return cudaGetLastError();
+}
 
 bool valid_shape(int32_t T, int32_t K, int64_t H, int32_t dtype) {
   return valid_tokens(T) && K >= 1 && K <= KF_SORT_MAX_TOP_K && H >= 1 && H <= KF_SORT_MAX_WIDTH && valid_dtype(dtype);
@@ -778,17 +788,14 @@ int kf_combine_tokens(const void* rows, int32_t dtype, int64_t rows_stride, int3
   if (num_rows == 0)   // no pair has a row
     return code(cudaMemsetAsync(output, 0, static_cast<size_t>(num_tokens) * width * elem_bytes(dtype), s));
   const bool vec = vec_rows(rows, rows_stride, width, dtype) && vec_rows(output, width, width, dtype);
+  const CombineArgs a{rows, nullptr, pair_row, nullptr, topk_weight, output, nullptr, rows_stride, num_tokens, top_k, width, num_rows};
   return code(dispatch_rows(dtype, vec, [&](auto t, auto v) {
     using E = ElemOf<decltype(t)>;
-    if constexpr (decltype(v)::value) {
-      return launch_pipe<E, false>(CombineArgs{rows, nullptr, pair_row, nullptr, topk_weight, output, nullptr, rows_stride,
-                                               num_tokens, top_k, width, num_rows}, sms, s);
-    } else {
-      combine_kernel<E><<<blocks(units, kRowWarps), kRowWarps * 32, 0, s>>>(
-          static_cast<const E*>(rows), rows_stride, num_rows, pair_row, topk_weight, num_tokens, top_k, width,
-          static_cast<E*>(output));
-      return cudaGetLastError();
-    }
+    constexpr bool kVec = decltype(v)::value;
+    if constexpr (kVec)
+      return launch_pipe<E, false>(a, sms, s);
+    else
+      return launch_combine<E>(a, s);
   }));
 }
 
@@ -817,19 +824,13 @@ int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype
     if (!grad_weight)   // the rows are not read: scatter the weighted gradient
       return launch_scatter<E, kVec, true>(grad_output, width, pair_row, row_pair, topk_weight, num_tokens, top_k, width,
                                            num_rows, grad_rows, false, s);
-    if constexpr (kVec) {
-      return launch_pipe<E, true>(CombineArgs{rows, grad_output, pair_row, row_pair, topk_weight, grad_rows, grad_weight,
-                                              rows_stride, num_tokens, top_k, width, num_rows}, sms, s);
-    } else {
-      // as many warps as share the slices evenly, kRowWarps at most
-      const int slices = (width + kSlice - 1) / kSlice, steps = (slices + kRowWarps - 1) / kRowWarps;
-      const int warps = (slices + steps - 1) / steps;
-      const unsigned grid = num_tokens + (grad_rows ? zero_blocks_for(num_rows) : 0u);
-      combine_backward_kernel<E><<<grid, warps * 32, 0, s>>>(
-          static_cast<const E*>(grad_output), static_cast<const E*>(rows), rows_stride, num_rows, pair_row, row_pair,
-          topk_weight, num_tokens, top_k, width, static_cast<E*>(grad_rows), grad_weight);
-      return cudaGetLastError();
-    }
+    const CombineArgs a{rows, grad_output, pair_row, row_pair, topk_weight, grad_rows, grad_weight, rows_stride, num_tokens, top_k, width, num_rows};
+    // fp32 takes the plain form: its steps are twice as long, and what it stores covers long runs
+    // as it is (4096 tokens, K = 8, 28672-byte rows: 323 us against 368 us; K = 4: 168 us against 181 us)
+    if constexpr (kVec && sizeof(E) == 2)
+      return launch_pipe<E, true>(a, sms, s);
+    else
+      return launch_combine_backward<E, kVec>(a, s);
   }));
 }
 
