@@ -37,14 +37,17 @@ __device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
   return e < -126 ? -126 : e;
 }
 
-// Magnitudes as unsigned keys in the type's own bits: larger magnitude, larger
-// key; infinities and NaN are at least kOddKey.  Two 16-bit keys share a word.
+// Magnitudes as keys in the type's own bits: larger magnitude, larger key.  Above
+// kRareKey a block needs more than the plain path: its scale is the type's last one
+// (1.75 * 2^127, or 1.75 * 2^15 of fp16, and above), or a value is not finite.
+// Two 16-bit keys share a word, and one instruction takes the larger of both, NaN
+// (key 0x7fff) winning.
 template <typename T>
-constexpr uint32_t kOddKey = 0x7f800000u;
+constexpr uint32_t kRareKey = 0x7f600000u;
 template <>
-constexpr uint32_t kOddKey<__nv_bfloat16> = 0x7f80u;
+constexpr uint32_t kRareKey<__nv_bfloat16> = 0x7f60u;
 template <>
-constexpr uint32_t kOddKey<__half> = 0x7c00u;
+constexpr uint32_t kRareKey<__half> = 0x7b00u;
 
 __device__ __forceinline__ uint32_t key_bits(uint32_t key, const float*) { return key; }   // the magnitude's fp32 bits
 __device__ __forceinline__ uint32_t key_bits(uint32_t key, const __nv_bfloat16*) { return key << 16; }
@@ -52,21 +55,14 @@ __device__ __forceinline__ uint32_t key_bits(uint32_t key, const __half*) {
   return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(key))));
 }
 
-// Largest key of elements 0..3 and of elements 4..7.
-template <typename T>
-__device__ __forceinline__ void max_keys(const Raw8<T>& r, uint32_t (&m)[2]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      m[h] = max(max(r.x[4 * h] & 0x7fffffffu, r.x[4 * h + 1] & 0x7fffffffu),
-                 max(r.x[4 * h + 2] & 0x7fffffffu, r.x[4 * h + 3] & 0x7fffffffu));
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t k = __vmaxu2(r.x[2 * h] & 0x7fff7fffu, r.x[2 * h + 1] & 0x7fff7fffu);
-      m[h] = max(k & 0xffffu, k >> 16);
-    }
-  }
+__device__ __forceinline__ uint32_t max2_keys(uint32_t a, uint32_t b, const __nv_bfloat16*) {
+  const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)),
+                                       __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max2_keys(uint32_t a, uint32_t b, const __half*) {
+  const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 // A slice of 256 columns = two blocks.  The vector form of 16-bit types has a block
@@ -74,31 +70,74 @@ __device__ __forceinline__ void max_keys(const Raw8<T>& r, uint32_t (&m)[2]) {
 template <typename T, bool kVec>
 constexpr bool kHalfWarp = kVec && sizeof(T) == 2;
 
-template <bool kHalf>
-__device__ __forceinline__ void block_max(uint32_t (&m)[2]) {
-  if (kHalf) {
-    uint32_t v = max(m[0], m[1]);
+// Largest keys of this lane's blocks (the same twice where a half-warp has one).
+template <typename T, bool kVec>
+__device__ __forceinline__ void block_keys(const Raw8<T>& r, uint32_t (&key)[2]) {
+  const T* type = nullptr;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, off));
-    m[0] = m[1] = v;
+    for (int h = 0; h < 2; ++h)
+      key[h] = __reduce_max_sync(0xffffffffu, max(max(r.x[4 * h] & 0x7fffffffu, r.x[4 * h + 1] & 0x7fffffffu),
+                                                  max(r.x[4 * h + 2] & 0x7fffffffu, r.x[4 * h + 3] & 0x7fffffffu)));
+  } else if constexpr (kHalfWarp<T, kVec>) {
+    uint32_t m = max2_keys(max2_keys(r.x[0], r.x[1], type), max2_keys(r.x[2], r.x[3], type), type);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) m = max2_keys(m, __shfl_xor_sync(0xffffffffu, m, off), type);
+    key[0] = key[1] = max(m & 0xffffu, m >> 16);
   } else {
-    m[0] = __reduce_max_sync(0xffffffffu, m[0]);
-    m[1] = __reduce_max_sync(0xffffffffu, m[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t m = max2_keys(r.x[2 * h], r.x[2 * h + 1], type);
+      key[h] = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    }
   }
 }
 
 // The same for two sets of values, whose 16-bit keys go through the shuffles in one word.
 template <typename T, bool kVec>
-__device__ __forceinline__ void block_max2(uint32_t (&a)[2], uint32_t (&b)[2]) {
+__device__ __forceinline__ void block_keys2(const Raw8<T>& a, const Raw8<T>& b, uint32_t (&ka)[2], uint32_t (&kb)[2]) {
   if constexpr (kHalfWarp<T, kVec>) {
-    uint32_t v = max(a[0], a[1]) | (max(b[0], b[1]) << 16);
+    const T* type = nullptr;
+    const uint32_t ma = max2_keys(max2_keys(a.x[0], a.x[1], type), max2_keys(a.x[2], a.x[3], type), type);
+    const uint32_t mb = max2_keys(max2_keys(b.x[0], b.x[1], type), max2_keys(b.x[2], b.x[3], type), type);
+    uint32_t m = max2_keys(__byte_perm(ma, mb, 0x5410), __byte_perm(ma, mb, 0x7632), type);
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, off));
-    a[0] = a[1] = v & 0xffffu;
-    b[0] = b[1] = v >> 16;
+    for (int off = 8; off >= 1; off >>= 1) m = max2_keys(m, __shfl_xor_sync(0xffffffffu, m, off), type);
+    ka[0] = ka[1] = m & 0xffffu;
+    kb[0] = kb[1] = m >> 16;
   } else {
-    block_max<false>(a);
-    block_max<false>(b);
+    block_keys<T, kVec>(a, ka);
+    block_keys<T, kVec>(b, kb);
+  }
+}
+
+// Blocks above kRareKey: the scale from the finite values, codes up to 240 under the type's last scale, NaN codes
+// for the others.
+template <typename T, bool kVec>
+__device__ __noinline__ void rare_blocks(float (&q)[8], int (&e)[2]) {
+  uint32_t a[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __float_as_uint(q[j]) & 0x7fffffffu;
+    if (b < 0x7f800000u) a[j >> 2] = max(a[j >> 2], b);
+  }
+  if (kHalfWarp<T, kVec>) {
+    uint32_t m = max(a[0], a[1]);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+    a[0] = a[1] = m;
+  } else {
+    a[0] = __reduce_max_sync(0xffffffffu, a[0]);
+    a[1] = __reduce_max_sync(0xffffffffu, a[1]);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) e[h] = block_exponent(a[h]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = q[j];
+    const float limit = e[j >> 2] == kTopExponent<T> ? 240.f : 448.f;
+    q[j] = fminf(fmaxf(v * pow2(-e[j >> 2]), -limit), limit);
+    if ((__float_as_uint(v) & 0x7fffffffu) >= 0x7f800000u) q[j] = __uint_as_float(0x7fffffffu);
   }
 }
 
@@ -106,32 +145,17 @@ __device__ __forceinline__ void block_max2(uint32_t (&a)[2], uint32_t (&b)[2]) {
 template <typename T, bool kVec>
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], const uint32_t (&key)[2], int (&e)[2]) {
   const T* type = nullptr;
-  uint32_t a[2] = {key_bits(key[0], type), key_bits(key[1], type)};
-  const bool odd = max(key[0], key[1]) >= kOddKey<T>;
-  if (__any_sync(0xffffffffu, odd)) {   // a value that is not finite: the scale comes from the others
-    a[0] = a[1] = 0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
-      if (b < 0x7f800000u) a[j >> 2] = max(a[j >> 2], b);
-    }
-    block_max<kHalfWarp<T, kVec>>(a);
-  }
-  e[0] = block_exponent(a[0]);
-  e[1] = kHalfWarp<T, kVec> ? e[0] : block_exponent(a[1]);
-  const float inv[2] = {pow2(-e[0]), pow2(-e[1])};
   float q[8];
+  if (__any_sync(0xffffffffu, max(key[0], key[1]) > kRareKey<T>)) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = v[j] * inv[j >> 2];
-  if (e[0] == kTopExponent<T> || e[1] == kTopExponent<T>) {
+    for (int j = 0; j < 8; ++j) q[j] = v[j];
+    rare_blocks<T, kVec>(q, e);
+  } else {
+    e[0] = block_exponent(key_bits(key[0], type));
+    e[1] = kHalfWarp<T, kVec> ? e[0] : block_exponent(key_bits(key[1], type));
+    const float inv[2] = {pow2(-e[0]), pow2(-e[1])};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (e[j >> 2] == kTopExponent<T>) q[j] = fminf(fmaxf(q[j], -240.f), 240.f);
-  }
-  if (odd) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if ((__float_as_uint(v[j]) & 0x7fffffffu) >= 0x7f800000u) q[j] = __uint_as_float(0x7fffffffu);
+    for (int j = 0; j < 8; ++j) q[j] = v[j] * inv[j >> 2];
   }
   return make_uint2(pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7]));
 }
@@ -201,8 +225,22 @@ __device__ __forceinline__ void decode8(uint2 c, const float (&s)[2], float (&v)
   }
 }
 
-// 1 / (1 + e^-x), both steps within 2 ulp; 0 where 1 + e^-x is beyond 2^126.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
+// 1 / (1 + e^-x); 0 where 1 + e^-x is beyond 2^126.  For fp32 rows expf and a
+// division of 2 ulp; for 16-bit rows, whose own rounding is 2^-9 or 2^-12, the
+// hardware's 2^y of y = -x log2 e (a rounding of y costs |x| 2^-24 of the result) and
+// reciprocal: 4 instructions instead of some 15, where the kernels are bound by
+// issuing them.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float x) {
+  if constexpr (sizeof(T) == 4) {
+    return __fdividef(1.0f, 1.0f + expf(-x));
+  } else {
+    float y, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + y));
+    return s;
+  }
+}
 
 // One warp per (row, group of kGroup slices), consecutive warps on consecutive
 // groups of a row: this warp's row and first slice.
@@ -242,8 +280,7 @@ __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x
     float v[8];
     uint32_t key[2];
     int e[2];
-    max_keys(raw[j], key);
-    block_max<kHalfWarp<T, kVec>>(key);
+    block_keys<T, kVec>(raw[j], key);
     to_floats(raw[j], v);
     const uint2 q = encode8<T, kVec>(v, key, e);
     store_codes<T, kVec>(codes + u.row * W + c, n, lane, q);
@@ -352,13 +389,11 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
     to_floats(ru[i], u);
     to_floats(rg[i], g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = u[j] * (g[j] * sigmoid(g[j]));
+    for (int j = 0; j < 8; ++j) a[j] = u[j] * (g[j] * sigmoid<T>(g[j]));
     store_raw8<T, kVec>(act + r * I + c, n, lane, from_floats<T>(a));
     if (codes == nullptr) continue;   // the activation alone
     uint32_t ku[2], kg[2];
-    max_keys(ru[i], ku);
-    max_keys(rg[i], kg);
-    block_max2<T, kVec>(ku, kg);
+    block_keys2<T, kVec>(ru[i], rg[i], ku, kg);
     uint8_t* cr = codes + r * 2 * I + c;
     uint8_t* er = exps + r * 2 * nb + c / kBlk;
     int e[2];
@@ -371,7 +406,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
   }
 }
 
-// From the kept values u, g and d = dL/dact: du = d g s, dg = d u s (1 + g (1 - s)), act = u g s, with s = sigmoid(g).
+// From the kept values u, g and d = dL/dact: du = d g s, dg = d u (s + g s (1 - s)), act = u g s, with s = sigmoid(g).
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ exps,
@@ -406,10 +441,10 @@ __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_
     decode8(qg[i], sg[i], g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float s = sigmoid(g[j]);
+      const float s = sigmoid<T>(g[j]);
       const float gs = g[j] * s;
       a[j] = u[j] * gs;
-      const float dg = d[j] * (u[j] * s * (1.0f + g[j] * (1.0f - s)));
+      const float dg = d[j] * u[j] * fmaf(gs, 1.0f - s, s);
       u[j] = d[j] * gs;
       g[j] = dg;
     }

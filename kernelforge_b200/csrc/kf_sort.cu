@@ -60,6 +60,17 @@ __global__ void __launch_bounds__(kHistThreads) order_hist_kernel(const int32_t*
   if (threadIdx.x < E) hist[static_cast<size_t>(blockIdx.x) * E + threadIdx.x] = h[threadIdx.x];
 }
 
+// Row q of those without a pair: zero_first[e] is the first such row of expert e's segment (entry kEG: of the
+// buffer's rest), zero_upto[e] how many there are up to its end.
+__device__ __forceinline__ int64_t zero_row(const int32_t* zero_first, const int32_t* zero_upto, int q) {
+  int lo = 0, hi = kEG;   // the first entry whose zero_upto is above q
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (zero_upto[mid] > q) hi = mid; else lo = mid + 1;
+  }
+  return static_cast<int64_t>(zero_first[lo]) + q - (lo > 0 ? zero_upto[lo - 1] : 0);
+}
+
 struct PlaceArgs {
   const int32_t* ids;
   const int32_t* hist;   // [nchunk][E]
@@ -69,28 +80,21 @@ struct PlaceArgs {
   int32_t *pair_row, *row_pair, *counts, *starts;
 };
 
-// Places and copies: block b owns the tokens [b T / G, (b + 1) T / G).
+// Places the pairs: block b owns the tokens [b T / G, (b + 1) T / G).
 //
 // Counting.  Each block finds, for every expert, the pairs of the whole call and
 // those before its own first token: from the histogram's rows and the ids between
-// the last chunk border and its first token, or in small calls from all ids.  So
+// the last chunk border and its first token, or in smaller calls from all ids.  So
 // no block waits for another, and the order needs one launch or two.
 // Ranks.  A pair's row is its expert's next row, plus the pairs of its expert in
 // the block's earlier warps, plus those in lower lanes of its own warp: stable and
 // without atomics on the order.
-// Rows (kCopy; small calls, where one launch is worth more than the last of the
-// bandwidth).  Each token's row is read once and stored once per pair, 256 columns
-// per warp and step, four steps' loads in flight.  Rows that no pair has -- the
-// ends of the segments and the rest of the buffer -- are shared by all blocks.
-template <typename T, bool kVec, bool kCopy>
-__global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const PlaceArgs a, const T* __restrict__ x,
-                                                                        T* __restrict__ rows) {
-  if (!kCopy) grid_dep_trigger();
+__global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const PlaceArgs a) {
+  grid_dep_trigger();
   __shared__ int32_t total[kEG], before[kEG];        // before becomes the next row of each expert
   __shared__ int32_t zero_first[kEG + 1];            // first row of expert e's padding; the last entry: the buffer's rest
   __shared__ int32_t zero_upto[kEG + 1];             // padding rows of experts <= e
   __shared__ uint16_t warp_count[kPlaceWarps][kEG];
-  __shared__ int32_t srow[kPlaceThreads];
   __shared__ int32_t warp_sum[2][kEG / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = gridDim.x;
@@ -174,13 +178,12 @@ __global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const Pl
     if (tid == kEG - 1) zero_upto[kEG] = pads_incl + a.R - zero_first[kEG];
   }
 
-  const int slices = (a.H + kSlice - 1) / kSlice;
   const int round_tokens = kPlaceThreads / a.K;
   for (int r0 = t0; r0 < t1; r0 += round_tokens) {
     const int ntok = min(round_tokens, t1 - r0), npair = ntok * a.K;
     const int nwarp = (npair + 31) / 32;
     for (int i = tid; i < nwarp * (kEG / 2); i += kPlaceThreads) reinterpret_cast<uint32_t*>(warp_count)[i] = 0u;
-    __syncthreads();   // also: zero_upto, before, and the previous round's reads of srow
+    __syncthreads();   // also: zero_upto and before
     const int p = r0 * a.K + tid;
     int e = -1, rank = 0;
     if (warp < nwarp) {
@@ -206,61 +209,141 @@ __global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const Pl
         row = before[e] + warp_count[warp][e] + rank;
         if (row >= a.R) row = -1;
       }
-      srow[tid] = row;
       a.pair_row[p] = row;
       if (row >= 0) a.row_pair[row] = p;
     }
     __syncthreads();
     if (tid < kEG) before[tid] += total[tid];
 
-    if constexpr (!kCopy) continue;
-    const int units = ntok * slices;
-    constexpr int kStep = 4;
-    int i = warp / slices, sl = warp % slices;   // this warp's next unit: token r0 + i, slice sl
-    for (int u = warp; u < units; u += kStep * kPlaceWarps) {
-      Raw8<T> v[kStep];
-      int ti[kStep], tc[kStep];
-#pragma unroll
-      for (int j = 0; j < kStep; ++j) {
-        ti[j] = i;
-        tc[j] = sl * kSlice;
-        if (u + j * kPlaceWarps < units)
-          v[j] = load_raw8<T, kVec>(x + static_cast<int64_t>(r0 + i) * a.stride + tc[j], a.H - tc[j], lane);
-        sl += kPlaceWarps;
-        while (sl >= slices) {
-          sl -= slices;
-          ++i;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kStep; ++j) {
-        if (u + j * kPlaceWarps >= units) break;
-        for (int k = 0; k < a.K; ++k) {
-          const int row = srow[ti[j] * a.K + k];
-          if (row >= 0) store_raw8<T, kVec>(rows + static_cast<int64_t>(row) * a.H + tc[j], a.H - tc[j], lane, v[j]);
-        }
-      }
-    }
   }
 
   __syncthreads();   // zero_upto (a block without tokens)
   const int zeros = zero_upto[kEG];
-  // kCopy: a block per row without a pair; else a thread per row
-  for (int q = kCopy ? blockIdx.x : blockIdx.x * kPlaceThreads + tid; q < zeros; q += kCopy ? G : G * kPlaceThreads) {
-    int lo = 0, hi = kEG;   // the first entry whose zero_upto is above q
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (zero_upto[mid] > q) hi = mid; else lo = mid + 1;
+  for (int q = blockIdx.x * kPlaceThreads + tid; q < zeros; q += G * kPlaceThreads)
+    a.row_pair[zero_row(zero_first, zero_upto, q)] = -1;
+}
+
+// Small calls (at most kSmallPairs pairs, few rows) in one launch.  Every block
+// ranks all pairs -- a call's worth of ids is a few loads per thread -- and then
+// copies its share of the (token, slice) units and zeroes its share of the rows
+// without a pair; a warp's first unit is on its way from memory meanwhile.
+constexpr int kSmallThreads = 256;
+constexpr int kSmallPairs = 1024;
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const PlaceArgs a, const T* __restrict__ x,
+                                                                   T* __restrict__ rows) {
+  constexpr int kWarps = kSmallThreads / 32, kRounds = kSmallPairs / kSmallThreads;
+  __shared__ uint16_t warp_count[kSmallPairs / 32][kEG];
+  __shared__ int32_t first[kEG], zero_first[kEG + 1], zero_upto[kEG + 1];
+  __shared__ int32_t srow[kSmallPairs];
+  __shared__ int2 warp_sum[kWarps];
+  __shared__ int zeros;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n = a.T * a.K, nwarp = (n + 31) / 32;
+  const int slices = (a.H + kSlice - 1) / kSlice, units = a.T * slices;
+  const int gw = blockIdx.x * kWarps + warp, nw = gridDim.x * kWarps;
+
+  Raw8<T> v = {};
+  if (gw < units) {
+    const int t = gw / slices, c = (gw - t * slices) * kSlice;
+    v = load_raw8<T, kVec>(x + static_cast<int64_t>(t) * a.stride + c, a.H - c, lane);
+  }
+  int e[kRounds], rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int p = r * kSmallThreads + tid;
+    e[r] = p < n ? local_expert(a.ids[p], a.offset, a.E) : -1;
+  }
+  for (int i = tid; i < nwarp * (kEG / 2); i += kSmallThreads) reinterpret_cast<uint32_t*>(warp_count)[i] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if (r * kSmallThreads >= n) break;
+    const unsigned same = __match_any_sync(0xffffffffu, e[r]);
+    rank[r] = __popc(same & ((1u << lane) - 1u));
+    if (e[r] >= 0 && rank[r] == 0) warp_count[r * kWarps + warp][e[r]] = static_cast<uint16_t>(__popc(same));
+  }
+  __syncthreads();
+  // thread e owns expert e: its pairs in earlier warps, its segment, and the rows without a pair up to its end
+  static_assert(kSmallThreads == kEG, "a thread per expert");
+  int count = 0;
+  for (int w = 0; w < nwarp; ++w) {
+    const int c = warp_count[w][tid];
+    warp_count[w][tid] = static_cast<uint16_t>(count);
+    count += c;
+  }
+  const int padded = (count + a.align - 1) / a.align * a.align;
+  int2 incl = make_int2(padded, count);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int px = __shfl_up_sync(0xffffffffu, incl.x, off), py = __shfl_up_sync(0xffffffffu, incl.y, off);
+    if (lane >= off) {
+      incl.x += px;
+      incl.y += py;
     }
-    const int64_t row = zero_first[lo] + q - (lo > 0 ? zero_upto[lo - 1] : 0);
-    if (kCopy) {
-      const Raw8<T> z = {};
-      for (int s = warp; s < slices; s += kPlaceWarps)
-        store_raw8<T, kVec>(rows + row * a.H + s * kSlice, a.H - s * kSlice, lane, z);
-      if (tid == 0) a.row_pair[row] = -1;
-    } else {
-      a.row_pair[row] = -1;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) {
+    incl.x += warp_sum[w].x;
+    incl.y += warp_sum[w].y;
+  }
+  const int start = incl.x - padded, end = min(incl.x, a.R);
+  const int live = start < a.R ? min(count, a.R - start) : 0;      // rows of this expert inside the buffer
+  first[tid] = start;
+  zero_first[tid] = min(start, a.R) + live;
+  // the experts before this one lie inside the buffer if this one starts in it; those past the end have no rows to zero
+  const int upto = start < a.R ? end - (incl.y - count + live) : 0x7fffffff;
+  zero_upto[tid] = upto;
+  if (tid == kEG - 1) {
+    zero_first[kEG] = end;
+    zero_upto[kEG] = 0x7fffffff;
+    if (incl.x < a.R) zeros = a.R - incl.y;                        // everything fits, and the buffer's rest is empty
+  }
+  if (start < a.R && incl.x >= a.R) zeros = upto;                  // the expert at the buffer's end
+  if (tid == 0 && a.R == 0) zeros = 0;
+  if (blockIdx.x == 0 && tid < a.E) {
+    a.counts[tid] = count;
+    a.starts[tid] = min(start, a.R);
+    if (tid == a.E - 1) a.starts[a.E] = end;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int p = r * kSmallThreads + tid;
+    if (p < n) {
+      int row = -1;
+      if (e[r] >= 0) {
+        row = first[e[r]] + warp_count[r * kWarps + warp][e[r]] + rank[r];
+        if (row >= a.R) row = -1;
+      }
+      srow[p] = row;
+      if (blockIdx.x == 0) {
+        a.pair_row[p] = row;
+        if (row >= 0) a.row_pair[row] = p;
+      }
     }
+  }
+  __syncthreads();
+  for (int u = gw; u < units; u += nw) {
+    const int t = u / slices, c = (u - t * slices) * kSlice;
+    if (u != gw) v = load_raw8<T, kVec>(x + static_cast<int64_t>(t) * a.stride + c, a.H - c, lane);
+    for (int k = 0; k < a.K; ++k) {
+      const int row = srow[t * a.K + k];
+      if (row >= 0) store_raw8<T, kVec>(rows + static_cast<int64_t>(row) * a.H + c, a.H - c, lane, v);
+    }
+  }
+  const Raw8<T> z = {};
+  const int nz = zeros;
+  int q = gw / slices, s = gw - q * slices;
+  while (q < nz) {
+    const int64_t row = zero_row(zero_first, zero_upto, q);
+    store_raw8<T, kVec>(rows + row * a.H + s * kSlice, a.H - s * kSlice, lane, z);
+    if (s == 0 && lane == 0) a.row_pair[row] = -1;
+    s += nw;
+    q += s / slices;
+    s %= slices;
   }
 }
 
@@ -303,17 +386,14 @@ __global__ void __launch_bounds__(kScatterWarps * 32) scatter_rows_kernel(
   const int sub = warp / warps;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + sub;
   const bool live = t < T_;
-  bool first = true;
+  grid_dep_wait();
   PairLane mine{-1, 0.f};
+  if (live) mine = load_pair(pair_row, weight, t, K, R, lane);
+  if (!__any_sync(0xffffffffu, mine.row >= 0)) return;   // a token of other ranks' experts: its row is not read
   for (int c = (warp - sub * warps) * kSlice; c < H; c += 2 * warps * kSlice) {
     const int c2 = c + warps * kSlice;
-    const Raw8<T> v0 = load_raw8<T, kVec>(x + (live ? t * stride : 0) + c, live ? H - c : 0, lane);
-    const Raw8<T> v1 = load_raw8<T, kVec>(x + (live ? t * stride : 0) + c2, live ? H - c2 : 0, lane);
-    if (first) {   // the order may still be on its way; x is not
-      grid_dep_wait();
-      if (live) mine = load_pair(pair_row, weight, t, K, R, lane);
-      first = false;
-    }
+    const Raw8<T> v0 = load_raw8<T, kVec>(x + t * stride + c, H - c, lane);
+    const Raw8<T> v1 = load_raw8<T, kVec>(x + t * stride + c2, H - c2, lane);
     for (int k = 0; k < K; ++k) {
       const int row = __shfl_sync(0xffffffffu, mine.row, k);
       if (row < 0) continue;
@@ -685,8 +765,8 @@ bool valid_shape(int32_t T, int32_t K, int64_t H, int32_t dtype) {
   return valid_tokens(T) && K >= 1 && K <= KF_SORT_MAX_TOP_K && H >= 1 && H <= KF_SORT_MAX_WIDTH && valid_dtype(dtype);
 }
 
-// Calls whose rows are at most this many bytes in all are placed and copied in one launch.
-constexpr int64_t kFusedBytes = 8 << 20;
+// Small calls whose rows are at most this many bytes in all are sorted in one launch.
+constexpr int64_t kSmallBytes = 16 << 20;
 
 template <typename P>
 using ElemOf = std::remove_const_t<std::remove_pointer_t<P>>;
@@ -704,7 +784,7 @@ size_t kf_sort_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t num_ex
   if (!valid_tokens(num_tokens) || top_k < 1 || top_k > KF_SORT_MAX_TOP_K || num_experts < 1 || num_experts > kEG)
     return 0;
   const OrderPlan plan = plan_order(num_tokens, top_k);
-  return static_cast<size_t>(plan.nchunk > 0 ? plan.nchunk : 1) * num_experts * sizeof(int32_t);
+  return static_cast<size_t>(plan.nchunk) * num_experts * sizeof(int32_t);
 }
 
 int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t* topk_idx, int32_t num_tokens,
@@ -720,7 +800,7 @@ int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t
   if (!counts || !starts || (num_tokens > 0 && (!x || !topk_idx || !pair_row)) || (num_rows > 0 && (!rows || !row_pair)))
     return KF_ERR_INVALID_ARGUMENT;
   const size_t need = kf_sort_workspace_bytes(num_tokens, top_k, num_experts);
-  if (!workspace) return KF_ERR_INVALID_ARGUMENT;
+  if (need && !workspace) return KF_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < need) return KF_ERR_WORKSPACE_TOO_SMALL;
   int sms = 0;
   const int rc = device_ready(&sms);
@@ -751,22 +831,27 @@ int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t
   }
   const int slices = (width + kSlice - 1) / kSlice;
   const bool vec = vec_rows(x, x_stride, width, dtype) && vec_rows(rows, width, width, dtype);
-  const bool fused = static_cast<int64_t>(num_rows) * width * static_cast<int64_t>(elem_bytes(dtype)) <= kFusedBytes;
-  // a block per SM; fewer where there is less than a token, or a step of every warp's zeroing, for each
-  const int64_t work = std::max<int64_t>(num_tokens, static_cast<int64_t>(num_rows) * slices / kPlaceWarps);
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, work)));
+  const bool small = num_tokens * top_k <= kSmallPairs &&
+                     static_cast<int64_t>(num_rows) * width * static_cast<int64_t>(elem_bytes(dtype)) <= kSmallBytes;
   return code(dispatch_rows(dtype, vec, [&](auto t, auto v) {
     using E = ElemOf<decltype(t)>;
     constexpr bool kVec = decltype(v)::value;
-    auto* kernel = fused ? place_tokens_kernel<E, kVec, true> : place_tokens_kernel<E, kVec, false>;
+    if (small) {
+      // a unit per warp, and up to eight of zeroing; two blocks per SM at most
+      const int64_t units = std::max<int64_t>(static_cast<int64_t>(num_tokens) * slices, static_cast<int64_t>(num_rows) * slices / 8);
+      const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * sms, (units + 7) / 8)));
+      sort_small_kernel<E, kVec><<<grid, kSmallThreads, 0, s>>>(a, static_cast<const E*>(x), static_cast<E*>(rows));
+      return cudaGetLastError();
+    }
     cudaError_t e;
+    const int grid = std::min(sms, std::max(1, num_tokens));
     if (plan.nchunk) {
-      e = launch_chained(kernel, dim3(grid), dim3(kPlaceThreads), 0, s, a, static_cast<const E*>(x), static_cast<E*>(rows));
+      e = launch_chained(place_tokens_kernel, dim3(grid), dim3(kPlaceThreads), 0, s, a);
     } else {
-      kernel<<<grid, kPlaceThreads, 0, s>>>(a, static_cast<const E*>(x), static_cast<E*>(rows));
+      place_tokens_kernel<<<grid, kPlaceThreads, 0, s>>>(a);
       e = cudaGetLastError();
     }
-    if (fused || e != cudaSuccess) return e;
+    if (e != cudaSuccess) return e;
     return launch_scatter<E, kVec, false>(x, x_stride, pair_row, row_pair, nullptr, num_tokens, top_k, width, num_rows,
                                           rows, true, s);
   }));

@@ -136,7 +136,8 @@ variable_list sort_forward(const Tensor& x, const Tensor& ids, const SortArgs& a
          starts = at::empty({a.experts + 1}, i32);
   const size_t need = kf_sort_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(K),
                                               static_cast<int32_t>(a.experts));
-  Tensor ws = at::empty({static_cast<int64_t>(need)}, ids.options().dtype(at::kByte));
+  Tensor ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, ids.options().dtype(at::kByte));
   check_rc(kf_sort_tokens(ptr(x), dtype_of(x, "x"), x.stride(0), ids.const_data_ptr<int32_t>(), static_cast<int32_t>(T),
                           static_cast<int32_t>(K), static_cast<int32_t>(H), static_cast<int32_t>(a.experts),
                           static_cast<int32_t>(a.offset), static_cast<int32_t>(a.align), static_cast<int32_t>(a.rows),

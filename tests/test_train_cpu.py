@@ -112,7 +112,7 @@ def _sort(**kw):
                                  dict(E=0), dict(E=257), dict(off=-1), dict(off=249), dict(align=0), dict(align=1025),
                                  dict(align=16, R=24), dict(R=-1), dict(R=(1 << 30) + 1), dict(dtype=3), dict(dtype=-1), dict(stride=-1),
                                  dict(x=NULL), dict(ids=NULL), dict(rows=NULL), dict(pr=NULL), dict(rp=NULL),
-                                 dict(cnt=NULL), dict(st=NULL), dict(ws=NULL)])
+                                 dict(cnt=NULL), dict(st=NULL), dict(T=65536, R=65536 * 2, ws=NULL)])
 def test_sort_refuses_bad_arguments_before_device_work(bad):
     assert _sort(**bad) == 1
 
@@ -121,7 +121,7 @@ def test_sort_refuses_a_small_workspace_and_sizes_it():
     lib = B.library()
     lib.kf_sort_workspace_bytes.restype = sz
     lib.kf_sort_workspace_bytes.argtypes = [i32, i32, i32]
-    assert 0 < lib.kf_sort_workspace_bytes(0, 1, 1) <= lib.kf_sort_workspace_bytes(4096, 8, 256)
+    assert lib.kf_sort_workspace_bytes(16, 8, 256) == 0 < lib.kf_sort_workspace_bytes(4096, 8, 256) < lib.kf_sort_workspace_bytes(65536, 8, 256)
     assert lib.kf_sort_workspace_bytes(1, 0, 1) == lib.kf_sort_workspace_bytes(1, 17, 1) == 0
     assert lib.kf_sort_workspace_bytes(1, 1, 257) == lib.kf_sort_workspace_bytes(-1, 1, 1) == 0
     assert _sort(T=65536, K=8, R=65536 * 8, wsb=16) == 2
