@@ -241,15 +241,15 @@ __device__ __forceinline__ void zero_rows(const int32_t* __restrict__ row_pair, 
 // Blocks for it behind a grid that does something else: two per SM, or one per 64 rows.
 inline unsigned zero_blocks_for(int R) { return static_cast<unsigned>(R < 64 * 296 ? (R + 63) / 64 : 296); }
 
-// Warps per token and tokens per block for `slices` slices of a row, two per warp.
+// Warps per token and tokens per block for `slices` slices of a row, `per` of them per warp.
 constexpr int kScatterWarps = 16;
 struct ScatterPlan {
   int warps, tokens;
 };
-inline ScatterPlan plan_scatter(int slices) {
-  const int per = (slices + 1) / 2;
-  const int steps = (per + kScatterWarps - 1) / kScatterWarps;
-  const int warps = (per + steps - 1) / steps;
+inline ScatterPlan plan_scatter(int slices, int per) {
+  const int need = (slices + per - 1) / per;
+  const int steps = (need + kScatterWarps - 1) / kScatterWarps;
+  const int warps = (need + steps - 1) / steps;
   return ScatterPlan{warps, warps > 8 ? 1 : 8 / warps};
 }
 

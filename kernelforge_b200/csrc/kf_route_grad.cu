@@ -9,35 +9,46 @@
 // and zero for every other expert: the choice itself has no gradient, and the
 // bias enters the choice only.  The sigmoids are taken again from the logits.
 //
-// One warp per token.  Lanes 0..7 hold the chosen experts; the row of 256
-// gradients is written in full, lane l columns 4 l .. and 128 + 4 l .. .
+// Four tokens per warp, eight lanes each: lane 8 i + k holds choice k of token i.
+// The warp first zeroes its four rows of 256 gradients, 512 bytes per store, and
+// after a warp barrier each lane stores its choice's gradient into its row.
+// (Every lane of a warp per token comparing its own eight columns with the eight
+// ids was bound by issuing those compares: 6.8 us against 5.0 us at 16384 tokens.)
 #include "kf_internal.cuh"
 
 namespace kf {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kTokens = 4;   // per warp
 
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const float* __restrict__ logits,
                                                                   const int32_t* __restrict__ topk_idx,
                                                                   const float* __restrict__ grad_w, int T, float rsf,
                                                                   float* __restrict__ grad_logits) {
   const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  if (t >= T) return;
-  int e = -1;
-  float s = 0.f, c = 0.f, g = 0.f;
-  if (lane < kTopK) {
-    e = topk_idx[t * kTopK + lane];
-    if (e >= 0 && e < kEG) {
-      g = grad_w[t * kTopK + lane];
-      const float x = logits[t * kEG + e];
-      s = 1.0f / (1.0f + expf(-x));
-      c = 1.0f / (1.0f + expf(x));   // 1 - s without the cancellation
-    } else {
-      e = -1;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * kTokens;
+  const int64_t t = t0 + (lane >> 3);
+  if (t0 >= T) return;
+  const bool live = t < T;
+  int e = live ? topk_idx[t * kTopK + (lane & 7)] : -1;
+  float g = live ? grad_w[t * kTopK + (lane & 7)] : 0.f;
+  if (e < 0 || e >= kEG) {   // no choice
+    e = -1;
+    g = 0.f;
+  }
+  const float x = e >= 0 ? logits[t * kEG + e] : 0.f;
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    if (t0 + i < T) {
+      float4* row = reinterpret_cast<float4*>(grad_logits + (t0 + i) * kEG);
+      row[lane] = zero;
+      row[32 + lane] = zero;
     }
   }
+  const float s = e >= 0 ? 1.0f / (1.0f + expf(-x)) : 0.f;
+  const float c = 1.0f / (1.0f + expf(x));   // 1 - s without the cancellation
   float sum = s;
 #pragma unroll
   for (int off = 4; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -45,19 +56,23 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const float* _
   float mean = g * p;
 #pragma unroll
   for (int off = 4; off >= 1; off >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, off);
-  const float d = rsf * p * c * (g - mean);
-  float v[8] = {};
+  float d = rsf * p * c * (g - mean);
+  // an id that a token repeats (outside the routing's contract) gets the sum of its gradients, from its first lane
+  const unsigned mine = 0xffu << (lane & 24);
+  const unsigned same = __match_any_sync(0xffffffffu, e) & mine;
+  bool store = e >= 0;
+  if (__any_sync(0xffffffffu, store && (same & (same - 1)))) {
+    float all = 0.f;
 #pragma unroll
-  for (int k = 0; k < kTopK; ++k) {
-    const int ek = __shfl_sync(0xffffffffu, e, k);
-    const float dk = __shfl_sync(0xffffffffu, d, k);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (ek == (j >> 2) * 128 + lane * 4 + (j & 3)) v[j] += dk;
+    for (int k = 0; k < kTopK; ++k) {
+      const float dk = __shfl_sync(0xffffffffu, d, (lane & 24) + k);
+      if ((same >> ((lane & 24) + k)) & 1u) all += dk;
+    }
+    d = all;
+    store = store && lane == __ffs(same) - 1;
   }
-  float4* dst = reinterpret_cast<float4*>(grad_logits + t * kEG);
-  dst[lane] = make_float4(v[0], v[1], v[2], v[3]);
-  dst[32 + lane] = make_float4(v[4], v[5], v[6], v[7]);
+  __syncwarp();   // the zeroes come first
+  if (store) grad_logits[t * kEG + e] = d;
 }
 
 }  // namespace
@@ -75,8 +90,8 @@ extern "C" int kf_moe_route_backward(const float* routing_logits, const int32_t*
   int sms = 0;
   const int rc = device_ready(&sms);
   if (rc != KF_OK) return rc;
-  constexpr int warps = kThreads / 32;
-  route_backward_kernel<<<(num_tokens + warps - 1) / warps, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+  constexpr int tokens = kThreads / 32 * kTokens;
+  route_backward_kernel<<<(num_tokens + tokens - 1) / tokens, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
       routing_logits, topk_idx, grad_weight, num_tokens, routed_scaling_factor, grad_logits);
   return cudaGetLastError() == cudaSuccess ? KF_OK : KF_ERR_CUDA;
 }

@@ -533,7 +533,7 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
     const uint8_t* e = static_cast<const uint8_t*>(exponents);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (sorted) {
-      const ScatterPlan p = plan_scatter((width + kSlice - 1) / kSlice);
+      const ScatterPlan p = plan_scatter((width + kSlice - 1) / kSlice, 2);
       const unsigned nwarp = p.warps * p.tokens, token_blocks = (num_rows + p.tokens - 1) / p.tokens;
       restore8_sorted_kernel<E, decltype(v)::value><<<token_blocks + zero_blocks_for(out_rows), nwarp * 32, 0, s>>>(
           c, e, num_rows, width, pair_row, row_pair, top_k, out_rows, p.warps, p.tokens, token_blocks,
