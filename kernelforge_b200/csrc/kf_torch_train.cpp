@@ -3,6 +3,7 @@
 // stream of the tensors' device, and the autograd functions.  Scratch is taken per
 // call, so calls on several streams and captured graphs never share any.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -26,14 +27,15 @@ void check_cuda(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor on a B200 (sm_100a); no CPU fallback");
 }
 
-int dtype_of(const Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
+int dtype_of(at::ScalarType type, const char* name) {
+  switch (type) {
     case at::kBFloat16: return KF_DTYPE_BF16;
     case at::kHalf: return KF_DTYPE_F16;
     case at::kFloat: return KF_DTYPE_F32;
-    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32, got ", t.scalar_type());
+    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32, got ", type);
   }
 }
+int dtype_of(const Tensor& t, const char* name) { return dtype_of(t.scalar_type(), name); }
 
 // A 2-D row tensor of a supported type whose rows are dense (a copy is made of any other).
 Tensor expect_rows(const Tensor& t, const char* name) {
@@ -63,6 +65,12 @@ void* stream_of(const at::Device& dev) { return at::cuda::getCurrentCUDAStream(d
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// An output or scratch tensor, straight from the caching allocator: at decode sizes the
+// dispatcher's share of at::empty (half a microsecond a tensor) is a tenth of a call.
+Tensor new_tensor(at::IntArrayRef shape, at::ScalarType dtype, const at::Device& dev) {
+  return Tensor(at::detail::empty_cuda(shape, dtype, dev, std::nullopt));
+}
+
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 void refuse_double_backward(const char* what) {
@@ -90,7 +98,7 @@ Order expect_order(const Tensor& pair_row, const Tensor& row_pair, const at::Dev
 Tensor combine_forward(const Tensor& rows, const Tensor& pair_row, const Tensor& weight) {
   const at::Device dev = rows.device();
   c10::cuda::CUDAGuard guard(dev);
-  Tensor out = at::empty({pair_row.size(0), rows.size(1)}, rows.options());
+  Tensor out = new_tensor({pair_row.size(0), rows.size(1)}, rows.scalar_type(), dev);
   check_rc(kf_combine_tokens(ptr(rows), dtype_of(rows, "rows"), rows.stride(0), static_cast<int32_t>(rows.size(0)),
                              pair_row.const_data_ptr<int32_t>(),
                              weight.defined() ? weight.const_data_ptr<float>() : nullptr,
@@ -108,8 +116,8 @@ std::tuple<Tensor, Tensor> combine_backward_impl(const Tensor& grad_out, const T
   const int64_t H = grad_out.size(1);
   Tensor g = grad_out.contiguous();
   Tensor grad_rows, grad_weight;
-  if (need_rows) grad_rows = at::empty({R, H}, g.options());
-  if (need_weight) grad_weight = at::empty({T, K}, g.options().dtype(at::kFloat));
+  if (need_rows) grad_rows = new_tensor({R, H}, g.scalar_type(), dev);
+  if (need_weight) grad_weight = new_tensor({T, K}, at::kFloat, dev);
   check_rc(kf_combine_backward(ptr(g), ptr(rows), dtype_of(g, "grad_output"), rows.defined() ? rows.stride(0) : H,
                                static_cast<int32_t>(R), order.pair_row.const_data_ptr<int32_t>(),
                                order.row_pair.const_data_ptr<int32_t>(),
@@ -130,14 +138,13 @@ variable_list sort_forward(const Tensor& x, const Tensor& ids, const SortArgs& a
   const at::Device dev = x.device();
   c10::cuda::CUDAGuard guard(dev);
   const int64_t T = ids.size(0), K = ids.size(1), H = x.size(1);
-  const auto i32 = ids.options();
-  Tensor rows = at::empty({a.rows, H}, x.options());
-  Tensor pair_row = at::empty({T, K}, i32), row_pair = at::empty({a.rows}, i32), counts = at::empty({a.experts}, i32),
-         starts = at::empty({a.experts + 1}, i32);
+  Tensor rows = new_tensor({a.rows, H}, x.scalar_type(), dev);
+  Tensor pair_row = new_tensor({T, K}, at::kInt, dev), row_pair = new_tensor({a.rows}, at::kInt, dev),
+         counts = new_tensor({a.experts}, at::kInt, dev), starts = new_tensor({a.experts + 1}, at::kInt, dev);
   const size_t need = kf_sort_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(K),
                                               static_cast<int32_t>(a.experts));
   Tensor ws;
-  if (need) ws = at::empty({static_cast<int64_t>(need)}, ids.options().dtype(at::kByte));
+  if (need) ws = new_tensor({static_cast<int64_t>(need)}, at::kByte, dev);
   check_rc(kf_sort_tokens(ptr(x), dtype_of(x, "x"), x.stride(0), ids.const_data_ptr<int32_t>(), static_cast<int32_t>(T),
                           static_cast<int32_t>(K), static_cast<int32_t>(H), static_cast<int32_t>(a.experts),
                           static_cast<int32_t>(a.offset), static_cast<int32_t>(a.align), static_cast<int32_t>(a.rows),
@@ -266,7 +273,7 @@ Tensor route_backward(const Tensor& routing_logits, const Tensor& topk_idx, cons
   const Tensor ids = expect(topk_idx, "topk_idx", at::kInt, {T, KF_MOE_TOP_K}, dev);
   const Tensor g = expect(grad_weight, "grad_weight", at::kFloat, {T, KF_MOE_TOP_K}, dev);
   c10::cuda::CUDAGuard guard(dev);
-  Tensor out = at::empty({T, KF_MOE_GLOBAL_EXPERTS}, logits.options());
+  Tensor out = new_tensor({T, KF_MOE_GLOBAL_EXPERTS}, at::kFloat, dev);
   check_rc(kf_moe_route_backward(logits.const_data_ptr<float>(), ids.const_data_ptr<int32_t>(),
                                  g.const_data_ptr<float>(), static_cast<int32_t>(T),
                                  static_cast<float>(routed_scaling_factor), out.data_ptr<float>(), stream_of(dev)),
@@ -278,8 +285,8 @@ variable_list route_forward(const Tensor& logits, const Tensor& bias, double rsf
   const at::Device dev = logits.device();
   c10::cuda::CUDAGuard guard(dev);
   const int64_t T = logits.size(0);
-  Tensor ids = at::empty({T, KF_MOE_TOP_K}, logits.options().dtype(at::kInt));
-  Tensor w = at::empty({T, KF_MOE_TOP_K}, logits.options());
+  Tensor ids = new_tensor({T, KF_MOE_TOP_K}, at::kInt, dev);
+  Tensor w = new_tensor({T, KF_MOE_TOP_K}, at::kFloat, dev);
   check_rc(kf_moe_route(logits.const_data_ptr<float>(), bias.const_data_ptr(), static_cast<int32_t>(T),
                         static_cast<float>(rsf), ids.data_ptr<int32_t>(), w.data_ptr<float>(), stream_of(dev)),
            "kf_moe_route");
@@ -322,11 +329,11 @@ std::tuple<Tensor, Tensor> route(const Tensor& routing_logits, const Tensor& rou
 int64_t blocks_of(int64_t width) { return (width + KF_MOE_BLOCK - 1) / KF_MOE_BLOCK; }
 
 std::tuple<Tensor, Tensor> pack8(const Tensor& x_in) {
-  const Tensor x = expect_rows(x_in.detach(), "x");
+  const Tensor x = expect_rows(x_in, "x");
   check_num_rows(x.size(0), "number of rows");
   c10::cuda::CUDAGuard guard(x.device());
-  Tensor codes = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kFloat8_e4m3fn));
-  Tensor exps = at::empty({x.size(0), blocks_of(x.size(1))}, x.options().dtype(at::kByte));
+  Tensor codes = new_tensor({x.size(0), x.size(1)}, at::kFloat8_e4m3fn, x.device());
+  Tensor exps = new_tensor({x.size(0), blocks_of(x.size(1))}, at::kByte, x.device());
   check_rc(kf_pack8(ptr(x), dtype_of(x, "x"), x.stride(0), static_cast<int32_t>(x.size(0)),
                     static_cast<int32_t>(x.size(1)), ptr(codes), ptr(exps), stream_of(x.device())),
            "kf_pack8");
@@ -361,8 +368,9 @@ Tensor restore8(const Tensor& codes_in, const Tensor& exps_in, at::ScalarType dt
     out_rows = map.size(0);
     K = o.pair_row.size(1);
   }
-  Tensor out = at::empty({out_rows, codes.size(1)}, codes.options().dtype(dtype));
-  check_rc(kf_restore8(ptr(codes), ptr(exps), dtype_of(out, "kept.dtype"), static_cast<int32_t>(codes.size(0)),
+  const int code = dtype_of(dtype, "kept.dtype");
+  Tensor out = new_tensor({out_rows, codes.size(1)}, dtype, dev);
+  check_rc(kf_restore8(ptr(codes), ptr(exps), code, static_cast<int32_t>(codes.size(0)),
                        static_cast<int32_t>(codes.size(1)), pairs.defined() ? pairs.const_data_ptr<int32_t>() : nullptr,
                        map.defined() ? map.const_data_ptr<int32_t>() : nullptr,
                        static_cast<int32_t>(K), static_cast<int32_t>(out_rows), ptr(out), stream_of(dev)),
@@ -371,16 +379,16 @@ Tensor restore8(const Tensor& codes_in, const Tensor& exps_in, at::ScalarType dt
 }
 
 std::tuple<Tensor, Tensor, Tensor> swiglu_forward(const Tensor& h_in, bool keep) {
-  const Tensor h = expect_rows(h_in.detach(), "h");
+  const Tensor h = expect_rows(h_in, "h");
   TORCH_CHECK(h.size(1) % 2 == 0, "h must be [R, 2 I] = [up | gate], got shape ", h.sizes());
   check_num_rows(h.size(0), "number of rows");
   const int64_t R = h.size(0), I = h.size(1) / 2;
   c10::cuda::CUDAGuard guard(h.device());
-  Tensor act = at::empty({R, I}, h.options());
+  Tensor act = new_tensor({R, I}, h.scalar_type(), h.device());
   Tensor codes, exps;
   if (keep) {
-    codes = at::empty({R, 2 * I}, h.options().dtype(at::kFloat8_e4m3fn));
-    exps = at::empty({R, 2 * blocks_of(I)}, h.options().dtype(at::kByte));
+    codes = new_tensor({R, 2 * I}, at::kFloat8_e4m3fn, h.device());
+    exps = new_tensor({R, 2 * blocks_of(I)}, at::kByte, h.device());
   }
   check_rc(kf_swiglu_pack8(ptr(h), dtype_of(h, "h"), h.stride(0), static_cast<int32_t>(R), static_cast<int32_t>(I),
                            ptr(act), ptr(codes), ptr(exps), stream_of(h.device())),
@@ -393,13 +401,13 @@ std::tuple<Tensor, Tensor, Tensor> swiglu_pack8(const Tensor& h) { return swiglu
 std::tuple<Tensor, Tensor> swiglu_backward8(const Tensor& codes_in, const Tensor& exps_in, const Tensor& grad_act,
                                             bool need_act) {
   auto [codes, exps] = expect_kept(codes_in, exps_in, 2);
-  const Tensor g = expect_rows(grad_act.detach(), "grad_act");
+  const Tensor g = expect_rows(grad_act, "grad_act");
   const int64_t R = codes.size(0), I = codes.size(1) / 2;
   TORCH_CHECK(g.device() == codes.device() && g.size(0) == R && g.size(1) == I, "grad_act must be [", R, ", ", I,
               "] on ", codes.device(), ", got ", g.sizes(), " on ", g.device());
   c10::cuda::CUDAGuard guard(g.device());
-  Tensor grad_h = at::empty({R, 2 * I}, g.options()), act;
-  if (need_act) act = at::empty({R, I}, g.options());
+  Tensor grad_h = new_tensor({R, 2 * I}, g.scalar_type(), g.device()), act;
+  if (need_act) act = new_tensor({R, I}, g.scalar_type(), g.device());
   check_rc(kf_swiglu_backward8(ptr(codes), ptr(exps), ptr(g), dtype_of(g, "grad_act"), g.stride(0),
                                static_cast<int32_t>(R), static_cast<int32_t>(I), ptr(grad_h), ptr(act),
                                stream_of(g.device())),
