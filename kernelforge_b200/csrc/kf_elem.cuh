@@ -238,7 +238,7 @@ __device__ __forceinline__ void zero_rows(const int32_t* __restrict__ row_pair, 
     __syncthreads();   // the list is rewritten next
   }
 }
-// Blocks for it behind a grid that does something else: two per SM, or one per 64 rows.
+// Blocks for it at the front of a grid that does something else: two per SM, or one per 64 rows.
 inline unsigned zero_blocks_for(int R) { return static_cast<unsigned>(R < 64 * 296 ? (R + 63) / 64 : 296); }
 
 // Warps per token and tokens per block for `slices` slices of a row, `per` of them per warp.

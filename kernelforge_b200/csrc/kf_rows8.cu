@@ -321,21 +321,19 @@ __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __res
 
 // Rows in expert order: a block holds a token's row across its warps, two slices
 // each, decodes it once and stores it K times (as scatter_rows_kernel, whose reason
-// for one block per token holds here too).  Blocks past the tokens zero the rows of
-// no pair.
+// for one block per token holds here too).  The first blocks zero the rows of no pair.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int T_, int W,
     const int32_t* __restrict__ pair_row, const int32_t* __restrict__ row_pair, int K, int R, int warps, int tokens,
-    unsigned token_blocks, T* __restrict__ out) {
+    unsigned zero_blocks, T* __restrict__ out) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x >= token_blocks) {
-    zero_rows<T, kVec>(row_pair, static_cast<int64_t>(T_) * K, blockIdx.x - token_blocks, gridDim.x - token_blocks, R, W,
-                       out);
+  if (blockIdx.x < zero_blocks) {
+    zero_rows<T, kVec>(row_pair, static_cast<int64_t>(T_) * K, blockIdx.x, zero_blocks, R, W, out);
     return;
   }
   const int sub = warp / warps;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + sub;
+  const int64_t t = static_cast<int64_t>(blockIdx.x - zero_blocks) * tokens + sub;
   if (t >= T_) return;
   const int nb = (W + kBlk - 1) / kBlk;
   int mine = -1;
@@ -534,9 +532,9 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (sorted) {
       const ScatterPlan p = plan_scatter((width + kSlice - 1) / kSlice, 2);
-      const unsigned nwarp = p.warps * p.tokens, token_blocks = (num_rows + p.tokens - 1) / p.tokens;
-      restore8_sorted_kernel<E, decltype(v)::value><<<token_blocks + zero_blocks_for(out_rows), nwarp * 32, 0, s>>>(
-          c, e, num_rows, width, pair_row, row_pair, top_k, out_rows, p.warps, p.tokens, token_blocks,
+      const unsigned token_blocks = (num_rows + p.tokens - 1) / p.tokens, zero_blocks = zero_blocks_for(out_rows);
+      restore8_sorted_kernel<E, decltype(v)::value><<<zero_blocks + token_blocks, p.warps * p.tokens * 32, 0, s>>>(
+          c, e, num_rows, width, pair_row, row_pair, top_k, out_rows, p.warps, p.tokens, zero_blocks,
           static_cast<E*>(output));
     } else {
       restore8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, s>>>(c, e, num_rows, width, static_cast<E*>(output));
