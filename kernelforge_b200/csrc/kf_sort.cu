@@ -22,9 +22,9 @@ namespace {
 
 constexpr int kPlaceThreads = 1024;
 constexpr int kPlaceWarps = kPlaceThreads / 32;
-constexpr int kHistThreads = 256;
-constexpr int kMaxChunks = 128;      // histogram chunks of a large call: what each block of the placing kernel sums
-constexpr int kDirectPairs = 8192;   // calls of at most this many pairs need no histogram kernel
+constexpr int kHistThreads = 1024;
+constexpr int kMaxChunks = 64;      // histogram chunks of a large call: what each block of the placing kernel sums
+constexpr int kDirectPairs = 12288;  // calls of at most this many pairs need no histogram kernel (measured: even at about 12000 and 1.3 x slower at 32768)
 
 __device__ __forceinline__ int local_expert(int id, int offset, int E) {
   const unsigned le = static_cast<unsigned>(id) - static_cast<unsigned>(offset);
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kHistThreads) order_hist_kernel(const int32_t*
                                                                   int32_t* __restrict__ hist) {
   grid_dep_trigger();
   __shared__ int32_t h[kEG];
-  h[threadIdx.x] = 0;
+  if (threadIdx.x < kEG) h[threadIdx.x] = 0;
   __syncthreads();
   const int p0 = blockIdx.x * chunk_pairs, p1 = min(n, p0 + chunk_pairs);
   for (int p = p0 + threadIdx.x; p < p1; p += kHistThreads) {
@@ -445,18 +445,20 @@ cudaError_t launch_scatter(const void* x, int64_t stride, const int32_t* pair_ro
 // ---- the pipelined form, for 16-byte rows ----
 //
 // Both directions read every pair's row once (K times the output) and are bound by
-// memory.  A block of up to 14 warps (7 for fp32) works on one token at a time, each
-// warp on every W-th slice; a step's loads -- up to eight rows, and the output's
-// gradient in the backward pass -- go by cp.async straight to shared memory, into
-// the lane's own 16-byte slots, while the step before is summed: no barrier, no
-// registers held by loads in flight.  Blocks stay and loop over the tokens, as many
-// as fit the SMs.  Measured (4096 tokens, K = 8, 14336-byte rows of bf16): forward
-// 84 us = 6.3 TB/s against 99 us with the loads in registers, backward 160 us against
-// 191 us; in the backward pass one wide block per SM beats several narrow ones (172 us
-// with six blocks of four warps), as its stores cover longer runs of each row.
+// memory.  A block of up to 14 warps (7 for fp32, 10 in the backward pass) works on
+// one token at a time, each warp on every W-th slice; a step's loads -- up to eight
+// rows, and the output's gradient in the backward pass -- go by cp.async straight to
+// shared memory, into the lane's own 16-byte slots, while the step before is summed:
+// no barrier, no registers held by loads in flight.  Blocks stay and loop over the
+// tokens, as many as fit the SMs.  Measured (K = 8, bf16; 4096 tokens of 7168 columns
+// and 16384 of 2048): forward 81 and 91 us = 6.5 and 6.6 TB/s against 94 and 106 us
+// with the loads in registers, backward 168 and 206 us = 5.9 and 5.5 TB/s against 202
+// and 239 us.  One wide block per SM beats several narrow ones in the backward pass
+// (172 us against 158 us in a version without its other work), as its stores cover
+// longer runs of each row; more warps or a third stage change nothing.
 constexpr int kStages = 2;
-template <typename T>
-constexpr int kPipeWarps = sizeof(T) == 4 ? 7 : 14;
+template <typename T, bool kBackward>
+constexpr int kPipeWarps = sizeof(T) == 4 ? 7 : kBackward ? 10 : 14;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -494,11 +496,11 @@ struct CombineArgs {
 
 // kRows rows per step, kBatches steps per slice (K <= kRows * kBatches).
 template <typename T, int kRows, int kBatches, bool kBackward>
-__global__ void __launch_bounds__(kPipeWarps<T> * 32) combine_pipe_kernel(const CombineArgs a) {
+__global__ void __launch_bounds__(kPipeWarps<T, kBackward> * 32) combine_pipe_kernel(const CombineArgs a) {
   constexpr int kHalves = sizeof(T) / 2;                     // 16-byte accesses per lane and row
   constexpr int kSlots = kRows + (kBackward ? 1 : 0);        // the last one: the output's gradient
   extern __shared__ __align__(16) uint4 pipe_smem[];
-  __shared__ float part[2][kPipeWarps<T>][kRows * kBatches];
+  __shared__ float part[2][kPipeWarps<T, kBackward>][kRows * kBatches];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
   const uint4* mine = pipe_smem + static_cast<size_t>(warp) * kStages * kSlots * kHalves * 32 + lane;
   const uint32_t mine_s = smem_u32(mine);
@@ -507,20 +509,29 @@ __global__ void __launch_bounds__(kPipeWarps<T> * 32) combine_pipe_kernel(const 
   const int slices = (a.H + kSlice - 1) / kSlice;
 
   // the stream of steps to issue, kStages - 1 ahead of the ones summed: token, slice, batch
+  // and the pairs of its token, of the token before it (being summed while the stream
+  // is one step into the next) and of the token after it (on their way: looked at only
+  // when the stream gets there, as a warp waits at a load's first use)
   int it = blockIdx.x, is = warp, ib = 0;
-  auto row_of = [&](int t) {
-    int r = -1;
-    if (t < a.T && lane < a.K) r = a.pair_row[static_cast<int64_t>(t) * a.K + lane];
-    return r < a.R ? r : -1;
+  auto after = [&](int t) { return t + gridDim.x < static_cast<unsigned>(a.T) ? static_cast<int>(t + gridDim.x) : a.T; };
+  auto fetch = [&](int t) {
+    PairLane p{-1, 1.f};
+    if (t < a.T && lane < a.K) {
+      p.row = a.pair_row[static_cast<int64_t>(t) * a.K + lane];
+      if (a.weight) p.w = a.weight[static_cast<int64_t>(t) * a.K + lane];
+    }
+    return p;
   };
-  int row_now = row_of(it), row_next = row_of(it + gridDim.x < static_cast<unsigned>(a.T) ? it + gridDim.x : a.T);
+  auto checked = [&](PairLane p) { return p.row >= 0 && p.row < a.R ? p : PairLane{-1, 0.f}; };
+  PairLane before{-1, 0.f}, now = fetch(it), next = fetch(after(it));
+  now = checked(now);
   auto issue = [&](int stage) {
     if (it < a.T) {
       const int c = is * kSlice;
       const uint32_t dst = mine_s + stage * kSlots * kHalves * 512;
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int row = __shfl_sync(0xffffffffu, row_now, ib * kRows + j);
+        const int row = __shfl_sync(0xffffffffu, now.row, ib * kRows + j);
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
           const int col = c + vec_col<T>(lane, h);
@@ -541,9 +552,10 @@ __global__ void __launch_bounds__(kPipeWarps<T> * 32) combine_pipe_kernel(const 
         is += W;
         if (is >= slices) {
           is = warp;
-          it = it + gridDim.x < static_cast<unsigned>(a.T) ? it + gridDim.x : a.T;
-          row_now = row_next;
-          row_next = row_of(it + gridDim.x < static_cast<unsigned>(a.T) ? it + gridDim.x : a.T);
+          it = after(it);
+          before = now;
+          now = checked(next);
+          next = fetch(after(it));
         }
       }
     }
@@ -557,7 +569,8 @@ __global__ void __launch_bounds__(kPipeWarps<T> * 32) combine_pipe_kernel(const 
 
   int stage = 0, par = 0;
   for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
-    const PairLane pair = load_pair(a.pair_row, a.weight, t, a.K, a.R, lane);
+    const PairLane pair = it == t ? now : before;
+    const int out_row = a.out ? pair.row : -1;   // backward: where this lane's pair is stored
     float dot[kBatches][kRows] = {};
     for (int sl = warp; sl < slices; sl += W) {
       const int c = sl * kSlice, n = a.H - c;
@@ -581,13 +594,13 @@ __global__ void __launch_bounds__(kPipeWarps<T> * 32) combine_pipe_kernel(const 
           to_floats(slot_load<T>(slot + kRows * kHalves * 32), g);
 #pragma unroll
           for (int j = 0; j < kRows; ++j) {
-            const int row = __shfl_sync(0xffffffffu, pair.row, b * kRows + j);
+            const int row = __shfl_sync(0xffffffffu, out_row, b * kRows + j);
             const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
             float f[8];
             to_floats(slot_load<T>(slot + j * kHalves * 32), f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot[b][j] = fmaf(g[i], f[i], dot[b][j]);
-            if (a.out && row >= 0) {
+            if (row >= 0) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) f[i] = w * g[i];
               store_raw8<T, true>(static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
@@ -627,10 +640,10 @@ cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
   constexpr int kWarpBytes = kStages * (kRows + (kBackward ? 1 : 0)) * kSlice * static_cast<int>(sizeof(T));
   auto* kernel = combine_pipe_kernel<T, kRows, kBatches, kBackward>;
   // the warps that share the slices evenly, and blocks for about kPipeWarps warps on each SM
-  const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kPipeWarps<T> - 1) / kPipeWarps<T>;
+  const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kPipeWarps<T, kBackward> - 1) / kPipeWarps<T, kBackward>;
   const int warps = (slices + steps - 1) / steps;
-  const int target = kPipeWarps<T> * 8 / kRows, per_sm = std::max(1, (target + warps / 2) / warps);
-  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kWarpBytes * kPipeWarps<T>);
+  const int target = kPipeWarps<T, kBackward> * 8 / kRows, per_sm = std::max(1, (target + warps / 2) / warps);
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kWarpBytes * kPipeWarps<T, kBackward>);
   if (e != cudaSuccess) return e;
   const int grid = std::min(a.T, sms * per_sm);
   kernel<<<grid, warps * 32, kWarpBytes * warps, s>>>(a);
