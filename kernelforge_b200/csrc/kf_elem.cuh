@@ -208,7 +208,7 @@ __device__ __forceinline__ Raw8<T> from_floats(const float (&v)[8]) {
 // the listed rows together, a slice each.  The whole block calls it.
 constexpr int kZeroList = 512;
 template <typename T, bool kVec>
-__device__ __forceinline__ void zero_rows(const int32_t* __restrict__ row_pair, int64_t pairs, int part, int parts, int R,
+__device__ __forceinline__ void zero_rows(const int32_t* row_pair, int64_t pairs, int part, int parts, int R,
                                           int H, T* __restrict__ rows) {
   __shared__ int32_t list[kZeroList];
   __shared__ int listed;

@@ -102,8 +102,6 @@ inline RowLayout packed_layout(const void* rows) {
 
 // KF_OK on a B200, with its SM count (sets the current device up on first use).
 int device_ready(int* num_sms);
-// Lets a kernel use `bytes` of dynamic shared memory on the current device (once per kernel and device).
-cudaError_t allow_smem(const void* kernel, int bytes);
 
 // Every kernel of the layer's launch chain is launched with programmatic stream
 // serialization: it may start while its predecessor in the stream is finishing,

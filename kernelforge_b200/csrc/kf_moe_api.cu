@@ -8,7 +8,6 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
-#include <map>
 #include <mutex>
 #include <vector>
 
@@ -289,20 +288,6 @@ int run_front_small(const Workspace& w, void* ws, const float* logits, const voi
 }  // namespace
 
 int device_ready(int* num_sms) { return ensure_device(num_sms); }
-
-cudaError_t allow_smem(const void* kernel, int bytes) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int> allowed;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  int& now = allowed[{dev, kernel}];
-  if (now >= bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) now = bytes;
-  return e;
-}
 
 Workspace plan_workspace(int32_t T, int32_t E) {
   Workspace w{};

@@ -463,7 +463,8 @@ unsigned grid_of(int64_t R, int64_t W) {
   return units <= 0xffffffffll - kWarps ? static_cast<unsigned>((units + kWarps - 1) / kWarps) : 0u;
 }
 
-inline bool aligned(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+// `a`: a power of two; rows of a type begin at a multiple of its size
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 template <int N>
 struct IntTag {
@@ -502,7 +503,7 @@ int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, i
   if (!valid_rows(num_rows, width, dtype) || x_stride < 0) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return KF_OK;
   const unsigned grid = grid_of(num_rows, width);
-  if (!x || !codes || !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
+  if (!x || !codes || !exponents || !grid || !aligned(x, elem_bytes(dtype))) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(x, x_stride, width, dtype) && aligned(codes, 8);
   return launch(dtype, vec, width, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
@@ -523,7 +524,7 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
     return KF_ERR_INVALID_ARGUMENT;
   if (out_rows == 0) return KF_OK;
   const unsigned grid = grid_of(num_rows, width);
-  if (!output || (num_rows > 0 && !grid)) return KF_ERR_INVALID_ARGUMENT;
+  if (!output || (num_rows > 0 && !grid) || !aligned(output, elem_bytes(dtype))) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(output, width, width, dtype) && aligned(codes, 8);
   return launch(dtype, vec, width, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
@@ -548,6 +549,7 @@ int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_
   if (num_rows == 0) return KF_OK;
   const unsigned grid = grid_of(num_rows, inter);
   if (!h || !act || !codes != !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
+  if (!aligned(h, elem_bytes(dtype)) || !aligned(act, elem_bytes(dtype))) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(h, h_stride, inter, dtype) && vec_rows(act, inter, inter, dtype) && aligned(codes, 8);
   return launch(dtype, vec, inter, [&](auto t, auto v, auto g) {
     using E = ElemOf<decltype(t)>;
@@ -563,6 +565,8 @@ int kf_swiglu_backward8(const void* codes, const void* exponents, const void* gr
   if (num_rows == 0) return KF_OK;
   const unsigned grid = grid_of(num_rows, inter);
   if (!codes || !exponents || !grad_act || !grad_h || !grid) return KF_ERR_INVALID_ARGUMENT;
+  if (!aligned(grad_act, elem_bytes(dtype)) || !aligned(grad_h, elem_bytes(dtype)) || !aligned(act, elem_bytes(dtype)))
+    return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(grad_act, grad_stride, inter, dtype) && vec_rows(grad_h, inter, inter, dtype) &&
                    (!act || vec_rows(act, inter, inter, dtype)) && aligned(codes, 8);
   return launch(dtype, vec, inter, [&](auto t, auto v, auto g) {

@@ -12,6 +12,7 @@
 // The reference sorts and combines inside its kernel() only, for its own FP8
 // layer and without gradients (solution/triton/kernel.py:46-82, :1920-1925).
 #include <algorithm>
+#include <atomic>
 
 #include "kf_elem.cuh"
 #include "kf_internal.cuh"
@@ -354,8 +355,10 @@ struct PairLane {
   int row;
   float w;
 };
-__device__ __forceinline__ PairLane load_pair(const int32_t* __restrict__ pair_row, const float* __restrict__ weight,
-                                              int64_t t, int K, int R, int lane) {
+// (No __restrict__: the order may come from the kernel before, which a block starts
+// before it ends, so these loads must stay behind grid_dep_wait().)
+__device__ __forceinline__ PairLane load_pair(const int32_t* pair_row, const float* weight, int64_t t, int K, int R,
+                                              int lane) {
   PairLane p{-1, 0.f};
   if (lane < K) {
     p.row = pair_row[t * K + lane];
@@ -375,8 +378,8 @@ __device__ __forceinline__ PairLane load_pair(const int32_t* __restrict__ pair_r
 // 99 us against 88 us for 16384 tokens, 32 local experts and 24576 rows, a third empty).
 template <typename T, bool kVec, bool kWeighted, int kPer>
 __global__ void __launch_bounds__(kScatterWarps * 32) scatter_rows_kernel(
-    const T* __restrict__ x, int64_t stride, const int32_t* __restrict__ pair_row, const int32_t* __restrict__ row_pair,
-    const float* __restrict__ weight, int T_, int K, int H, int R, int warps, int tokens, unsigned zero_blocks,
+    const T* __restrict__ x, int64_t stride, const int32_t* pair_row, const int32_t* row_pair,
+    const float* weight, int T_, int K, int H, int R, int warps, int tokens, unsigned zero_blocks,
     T* __restrict__ rows) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (blockIdx.x < zero_blocks) {
@@ -643,8 +646,17 @@ cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
   const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kPipeWarps<T, kBackward> - 1) / kPipeWarps<T, kBackward>;
   const int warps = (slices + steps - 1) / steps;
   const int target = kPipeWarps<T, kBackward> * 8 / kRows, per_sm = std::max(1, (target + warps / 2) / warps);
-  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kWarpBytes * kPipeWarps<T, kBackward>);
+  // allowed once per device; a second thread that gets here first does the same again
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (dev >= 64 || !(allowed.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarpBytes * kPipeWarps<T, kBackward>);
+    if (e != cudaSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_release);
+  }
   const int grid = std::min(a.T, sms * per_sm);
   kernel<<<grid, warps * 32, kWarpBytes * warps, s>>>(a);
   return cudaGetLastError();
@@ -782,6 +794,9 @@ bool valid_shape(int32_t T, int32_t K, int64_t H, int32_t dtype) {
   return valid_tokens(T) && K >= 1 && K <= KF_SORT_MAX_TOP_K && H >= 1 && H <= KF_SORT_MAX_WIDTH && valid_dtype(dtype);
 }
 
+// Rows of a type begin at a multiple of its size (a null pointer does).
+bool elem_aligned(const void* p, int32_t dtype) { return reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype) == 0; }
+
 // Small calls whose rows are at most this many bytes in all are sorted in one launch.
 constexpr int64_t kSmallBytes = 16 << 20;
 
@@ -816,6 +831,7 @@ int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t
     return KF_ERR_INVALID_ARGUMENT;
   if (!counts || !starts || (num_tokens > 0 && (!x || !topk_idx || !pair_row)) || (num_rows > 0 && (!rows || !row_pair)))
     return KF_ERR_INVALID_ARGUMENT;
+  if (!elem_aligned(x, dtype) || !elem_aligned(rows, dtype)) return KF_ERR_INVALID_ARGUMENT;
   const size_t need = kf_sort_workspace_bytes(num_tokens, top_k, num_experts);
   if (need && !workspace) return KF_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < need) return KF_ERR_WORKSPACE_TOO_SMALL;
@@ -881,6 +897,7 @@ int kf_combine_tokens(const void* rows, int32_t dtype, int64_t rows_stride, int3
     return KF_ERR_INVALID_ARGUMENT;
   if (num_tokens == 0) return KF_OK;
   if (!pair_row || !output || (num_rows > 0 && !rows)) return KF_ERR_INVALID_ARGUMENT;
+  if (!elem_aligned(rows, dtype) || !elem_aligned(output, dtype)) return KF_ERR_INVALID_ARGUMENT;
   const int64_t units = static_cast<int64_t>(num_tokens) * ((width + kSlice - 1) / kSlice);
   if (units > 0xffffffffll - kRowWarps) return KF_ERR_INVALID_ARGUMENT;   // rows of terabytes
   int sms = 0;
@@ -909,6 +926,8 @@ int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype
   if (num_tokens > 0 && (!grad_output || !pair_row)) return KF_ERR_INVALID_ARGUMENT;
   if (grad_weight && num_rows > 0 && !rows) return KF_ERR_INVALID_ARGUMENT;
   if (grad_rows && num_rows > 0 && !row_pair) return KF_ERR_INVALID_ARGUMENT;
+  if (!elem_aligned(grad_output, dtype) || !elem_aligned(rows, dtype) || !elem_aligned(grad_rows, dtype))
+    return KF_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) grad_rows = nullptr;
   if (num_tokens == 0) grad_weight = nullptr;
   if (!grad_weight && !grad_rows) return KF_OK;

@@ -71,7 +71,24 @@ Tensor new_tensor(at::IntArrayRef shape, at::ScalarType dtype, const at::Device&
   return Tensor(at::detail::empty_cuda(shape, dtype, dev, std::nullopt));
 }
 
-bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Whether a call on `t` is recorded for autograd.  During a stream capture a leaf whose
+// gradient accumulator already lives on another stream -- an eager graph of the same
+// leaf is still alive -- is refused: the backward pass would make that stream wait for
+// the capturing one, which invalidates the capture inside the autograd engine.
+bool wants_grad(const Tensor& t) {
+  if (!at::GradMode::is_enabled() || !t.requires_grad()) return false;
+  if (t.is_leaf()) {
+    const at::cuda::CUDAStream now = at::cuda::getCurrentCUDAStream(t.device().index());
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(now.stream(), &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
+      const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
+      TORCH_CHECK(!acc || !acc->stream().has_value() || *acc->stream() == now.unwrap(),
+                  "a captured call on a leaf tensor whose eager autograd graph is still alive: release that graph "
+                  "first, or capture a detached copy that requires grad");
+    }
+  }
+  return true;
+}
 
 void refuse_double_backward(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is not twice differentiable (backward with create_graph=True)");
@@ -174,7 +191,7 @@ struct SortFn : public torch::autograd::Function<SortFn> {
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> sort_tokens(const Tensor& x_in, const Tensor& topk_idx,
                                                                int64_t num_experts, int64_t expert_offset,
-                                                               int64_t row_align, int64_t max_rows) {
+                                                               int64_t row_align, std::optional<int64_t> max_rows) {
   const Tensor x = expect_rows(x_in, "x");
   const int64_t T = x.size(0);
   TORCH_CHECK(topk_idx.dim() == 2 && topk_idx.size(0) == T && topk_idx.size(1) >= 1 &&
@@ -190,9 +207,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> sort_tokens(const Tensor& x_i
               row_align);
   const int64_t pairs = T * ids.size(1);
   int64_t rows = (pairs + std::min(pairs, num_experts) * (row_align - 1)) / row_align * row_align;
-  if (max_rows >= 0) {
-    TORCH_CHECK(max_rows % row_align == 0, "max_rows must be a multiple of row_align (", row_align, "), got ", max_rows);
-    rows = max_rows;
+  if (max_rows.has_value()) {
+    TORCH_CHECK(*max_rows >= 0 && *max_rows % row_align == 0, "max_rows must be a multiple of row_align (", row_align,
+                ") and not negative, got ", *max_rows);
+    rows = *max_rows;
   }
   check_num_rows(rows, "number of rows");
   variable_list o = wants_grad(x) ? SortFn::apply(x, ids, num_experts, expert_offset, row_align, rows)

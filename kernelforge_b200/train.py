@@ -16,9 +16,10 @@ order; ``swiglu_backward8`` returns the activation along with the gradient.
 
 Every call runs on the current stream of its tensors' device, allocates its outputs and
 scratch from torch's caching allocator and never synchronises, so it can be captured into
-a CUDA graph.  Errors raise ``RuntimeError``.  Sums are fp32 in a fixed order: equal inputs
-give equal bits.  The gradients are not differentiable again: a backward pass with
-``create_graph=True`` raises.
+a CUDA graph, after one call outside a capture (the library's set-up on a device).  A
+captured call on a leaf tensor that an eager autograd graph still holds raises.  Errors raise
+``RuntimeError``.  Sums are fp32 in a fixed order: equal inputs give equal bits.  The gradients
+are not differentiable again: a backward pass with ``create_graph=True`` raises.
 
 The reference has no training path; its routing, sort and combine are inside ``kernel``
 (``solution/triton/kernel.py:1842-1925``).
@@ -33,7 +34,11 @@ from . import binding as B
 
 
 class TokenOrder(NamedTuple):
-    """Where ``sort_tokens`` put each (token, choice) pair; all int32 on the tokens' device."""
+    """Where ``sort_tokens`` put each (token, choice) pair; all int32 on the tokens' device.
+
+    The operators take it as ``sort_tokens`` gave it.  In an order put together otherwise, rows and
+    pairs out of range count as none; rows that ``row_pair`` and ``pair_row`` disagree about are undefined.
+    """
     pair_row: torch.Tensor   # [T, K] row of each pair, -1 without one
     row_pair: torch.Tensor   # [R] pair t * K + k of each row, -1 without one
     counts: torch.Tensor     # [E] pairs of each local expert
@@ -78,10 +83,8 @@ def sort_tokens(x: torch.Tensor, topk_idx: torch.Tensor, num_experts: int, exper
     the end are dropped.  ``order.counts`` counts them still, so drops are visible.  An id that a
     token repeats is a pair of its own.
     """
-    if max_rows is not None and max_rows < 0:
-        raise ValueError("max_rows must not be negative")
     rows, pair_row, row_pair, counts, starts = B.extension().sort_tokens(
-        x, topk_idx, num_experts, expert_offset, row_align, -1 if max_rows is None else max_rows)
+        x, topk_idx, num_experts, expert_offset, row_align, max_rows)
     return rows, TokenOrder(pair_row, row_pair, counts, starts)
 
 

@@ -111,7 +111,7 @@ def _sort(**kw):
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(T=(1 << 24) + 1), dict(K=0), dict(K=17), dict(H=0), dict(H=(1 << 20) + 1),
                                  dict(E=0), dict(E=257), dict(off=-1), dict(off=249), dict(align=0), dict(align=1025),
                                  dict(align=16, R=24), dict(R=-1), dict(R=(1 << 30) + 1), dict(dtype=3), dict(dtype=-1), dict(stride=-1),
-                                 dict(x=NULL), dict(ids=NULL), dict(rows=NULL), dict(pr=NULL), dict(rp=NULL),
+                                 dict(x=NULL), dict(x=vp(257)), dict(rows=vp(258), dtype=2), dict(ids=NULL), dict(rows=NULL), dict(pr=NULL), dict(rp=NULL),
                                  dict(cnt=NULL), dict(st=NULL), dict(T=65536, R=65536 * 2, ws=NULL)])
 def test_sort_refuses_bad_arguments_before_device_work(bad):
     assert _sort(**bad) == 1
@@ -128,7 +128,7 @@ def test_sort_refuses_a_small_workspace_and_sizes_it():
 
 
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(K=0), dict(K=17), dict(H=0), dict(dtype=5), dict(R=-1), dict(pr=NULL),
-                                 dict(out=NULL), dict(rows=NULL), dict(stride=-3)])
+                                 dict(out=NULL), dict(out=vp(257)), dict(rows=NULL), dict(rows=vp(1)), dict(stride=-3)])
 def test_combine_refuses_bad_arguments_before_device_work(bad):
     a = dict(rows=SOME, dtype=0, stride=64, R=8, pr=SOME, w=NULL, T=4, K=2, H=64, out=SOME)
     a.update(bad)
@@ -155,7 +155,7 @@ def test_the_8_bit_entry_points_refuse_bad_arguments_before_device_work():
     lib.kf_swiglu_pack8.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp]
     lib.kf_swiglu_backward8.argtypes = [vp, vp, vp, i32, i64, i32, i32, vp, vp, vp]
     ok = (SOME, 0, 64, 4, 64, SOME, SOME, NULL)
-    for i, v in ((0, NULL), (1, 3), (2, -1), (3, -1), (4, 0), (4, (1 << 20) + 1), (5, NULL), (6, NULL)):
+    for i, v in ((0, NULL), (0, vp(33)), (1, 3), (2, -1), (3, -1), (4, 0), (4, (1 << 20) + 1), (5, NULL), (6, NULL)):
         assert lib.kf_pack8(*(v if j == i else a for j, a in enumerate(ok))) == 1
     ok = (SOME, SOME, 0, 4, 64, SOME, SOME, 2, 8, SOME, NULL)
     for i, v in ((0, NULL), (1, NULL), (2, 9), (3, -1), (3, (1 << 24) + 1), (4, 0), (5, NULL), (7, 0), (7, 17), (8, -1), (9, NULL)):
