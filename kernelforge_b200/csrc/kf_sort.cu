@@ -445,23 +445,12 @@ cudaError_t launch_scatter(const void* x, int64_t stride, const int32_t* pair_ro
 // ---------------------------------------------------------------- combine --
 
 
-// ---- the pipelined form, for 16-byte rows ----
+// ---- the pipelined forms, for 16-byte rows ----
 //
 // Both directions read every pair's row once (K times the output) and are bound by
-// memory.  A block of up to 14 warps (7 for fp32, 10 in the backward pass) works on
-// one token at a time, each warp on every W-th slice; a step's loads -- up to eight
-// rows, and the output's gradient in the backward pass -- go by cp.async straight to
-// shared memory, into the lane's own 16-byte slots, while the step before is summed:
-// no barrier, no registers held by loads in flight.  Blocks stay and loop over the
-// tokens, as many as fit the SMs.  Measured (K = 8, bf16; 4096 tokens of 7168 columns
-// and 16384 of 2048): forward 81 and 91 us = 6.5 and 6.6 TB/s against 94 and 106 us
-// with the loads in registers, backward 168 and 206 us = 5.9 and 5.5 TB/s against 202
-// and 239 us.  One wide block per SM beats several narrow ones in the backward pass
-// (172 us against 158 us in a version without its other work), as its stores cover
-// longer runs of each row; more warps or a third stage change nothing.
-constexpr int kStages = 2;
-template <typename T, bool kBackward>
-constexpr int kPipeWarps = sizeof(T) == 4 ? 7 : kBackward ? 10 : 14;
+// memory.  A warp's step is a slice of a token: its loads -- up to eight rows, and the
+// output's gradient in the backward pass -- go by cp.async straight to shared memory,
+// into the lane's own 16-byte slots, so they need no barrier and hold no registers.
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -470,12 +459,27 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// This lane's eight elements of a slot row (512 bytes per 16-byte access of a warp).
+// A slot row is 512 bytes per 16-byte access of a warp (one for 16-bit types, two for fp32).
+template <typename T>
+constexpr int kHalves = static_cast<int>(sizeof(T)) / 2;
+
+// Starts the copy of a slice (at column c of `row`, null for none) into a slot row; the rest of it becomes zeros.
+template <typename T>
+__device__ __forceinline__ void slot_copy(uint32_t slot, const T* row, const T* any, int c, int H, int lane) {
+#pragma unroll
+  for (int h = 0; h < kHalves<T>; ++h) {
+    const int col = c + vec_col<T>(lane, h);
+    const bool live = row != nullptr && col < H;
+    cp_async16(slot + h * 512, live ? row + col : any, live);
+  }
+}
+
+// This lane's eight elements of a slot row.
 template <typename T>
 __device__ __forceinline__ Raw8<T> slot_load(const uint4* slot) {
   Raw8<T> r;
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+  for (int i = 0; i < kHalves<T>; ++i) {
     const uint4 q = slot[i * 32];
     r.x[4 * i] = q.x;
     r.x[4 * i + 1] = q.y;
@@ -497,21 +501,28 @@ struct CombineArgs {
   int T, K, H, R;
 };
 
+// Forward.  A block of up to 14 warps (7 for fp32) stays and loops over tokens, as many
+// blocks as fit the SMs; each warp sums one step while the next one's rows arrive, and
+// the pairs of the token after that are on their way.  Measured (K = 8, bf16; 4096
+// tokens of 7168 columns and 16384 of 2048): 81 and 91 us = 6.5 and 6.6 TB/s, against
+// 94 and 106 us with the rows loaded to registers.
+constexpr int kForwardStages = 2;
+template <typename T>
+constexpr int kForwardWarps = sizeof(T) == 4 ? 7 : 14;
+
 // kRows rows per step, kBatches steps per slice (K <= kRows * kBatches).
-template <typename T, int kRows, int kBatches, bool kBackward>
-__global__ void __launch_bounds__(kPipeWarps<T, kBackward> * 32) combine_pipe_kernel(const CombineArgs a) {
-  constexpr int kHalves = sizeof(T) / 2;                     // 16-byte accesses per lane and row
-  constexpr int kSlots = kRows + (kBackward ? 1 : 0);        // the last one: the output's gradient
+template <typename T, int kRows, int kBatches>
+__global__ void __launch_bounds__(kForwardWarps<T> * 32) combine_pipe_kernel(const CombineArgs a) {
+  constexpr int kStages = kForwardStages;
+  constexpr int kStep = kRows * kHalves<T>;                  // 512-byte slots of a step
   extern __shared__ __align__(16) uint4 pipe_smem[];
-  __shared__ float part[2][kPipeWarps<T, kBackward>][kRows * kBatches];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-  const uint4* mine = pipe_smem + static_cast<size_t>(warp) * kStages * kSlots * kHalves * 32 + lane;
+  const uint4* mine = pipe_smem + static_cast<size_t>(warp) * kStages * kStep * 32 + lane;
   const uint32_t mine_s = smem_u32(mine);
   const T* rows = static_cast<const T*>(a.rows);
-  const T* dout = static_cast<const T*>(a.dout);
   const int slices = (a.H + kSlice - 1) / kSlice;
 
-  // the stream of steps to issue, kStages - 1 ahead of the ones summed: token, slice, batch
+  // the stream of steps to issue, kStages - 1 ahead of the ones summed: token, slice, batch;
   // and the pairs of its token, of the token before it (being summed while the stream
   // is one step into the next) and of the token after it (on their way: looked at only
   // when the stream gets there, as a warp waits at a load's first use)
@@ -530,25 +541,12 @@ __global__ void __launch_bounds__(kPipeWarps<T, kBackward> * 32) combine_pipe_ke
   now = checked(now);
   auto issue = [&](int stage) {
     if (it < a.T) {
-      const int c = is * kSlice;
-      const uint32_t dst = mine_s + stage * kSlots * kHalves * 512;
+      const uint32_t dst = mine_s + stage * kStep * 512;
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
         const int row = __shfl_sync(0xffffffffu, now.row, ib * kRows + j);
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const int col = c + vec_col<T>(lane, h);
-          const bool live = row >= 0 && col < a.H;
-          cp_async16(dst + (j * kHalves + h) * 512, rows + (live ? static_cast<int64_t>(row) * a.stride + col : 0), live);
-        }
-      }
-      if (kBackward) {
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const int col = c + vec_col<T>(lane, h);
-          const bool live = col < a.H;
-          cp_async16(dst + (kRows * kHalves + h) * 512, dout + (live ? static_cast<int64_t>(it) * a.H + col : 0), live);
-        }
+        slot_copy<T>(dst + j * kHalves<T> * 512, row >= 0 ? rows + static_cast<int64_t>(row) * a.stride : nullptr, rows,
+                     is * kSlice, a.H, lane);
       }
       if (++ib == kBatches) {
         ib = 0;
@@ -567,110 +565,200 @@ __global__ void __launch_bounds__(kPipeWarps<T, kBackward> * 32) combine_pipe_ke
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue(i);
 
-  if (kBackward && a.out)
-    zero_rows<T, true>(a.row_pair, static_cast<int64_t>(a.T) * a.K, blockIdx.x, gridDim.x, a.R, a.H, static_cast<T*>(a.out));
-
-  int stage = 0, par = 0;
+  int stage = 0;
   for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
     const PairLane pair = it == t ? now : before;
-    const int out_row = a.out ? pair.row : -1;   // backward: where this lane's pair is stored
-    float dot[kBatches][kRows] = {};
     for (int sl = warp; sl < slices; sl += W) {
-      const int c = sl * kSlice, n = a.H - c;
+      const int c = sl * kSlice;
       float acc[8] = {};
 #pragma unroll
       for (int b = 0; b < kBatches; ++b) {
         issue(stage == 0 ? kStages - 1 : stage - 1);
         cp_async_wait<kStages - 1>();   // the oldest step's copies, all of this lane's own
-        const uint4* slot = mine + stage * kSlots * kHalves * 32;
-        if (!kBackward) {
+        const uint4* slot = mine + stage * kStep * 32;
 #pragma unroll
-          for (int j = 0; j < kRows; ++j) {
-            const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
-            float f[8];
-            to_floats(slot_load<T>(slot + j * kHalves * 32), f);
+        for (int j = 0; j < kRows; ++j) {
+          const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
+          float f[8];
+          to_floats(slot_load<T>(slot + j * kHalves<T> * 32), f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
-          }
-        } else {
-          float g[8];
-          to_floats(slot_load<T>(slot + kRows * kHalves * 32), g);
-#pragma unroll
-          for (int j = 0; j < kRows; ++j) {
-            const int row = __shfl_sync(0xffffffffu, out_row, b * kRows + j);
-            const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
-            float f[8];
-            to_floats(slot_load<T>(slot + j * kHalves * 32), f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dot[b][j] = fmaf(g[i], f[i], dot[b][j]);
-            if (row >= 0) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = w * g[i];
-              store_raw8<T, true>(static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
-            }
-          }
+          for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
         }
         stage = stage + 1 == kStages ? 0 : stage + 1;
       }
-      if (!kBackward)
-        store_raw8<T, true>(static_cast<T*>(a.out) + static_cast<int64_t>(t) * a.H + c, n, lane, from_floats<T>(acc));
-    }
-    if (kBackward) {
-#pragma unroll
-      for (int b = 0; b < kBatches; ++b)
-#pragma unroll
-        for (int j = 0; j < kRows; ++j) {
-          float d = dot[b][j];
-#pragma unroll
-          for (int off = 16; off >= 1; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
-          if (lane == 0) part[par][warp][b * kRows + j] = d;
-        }
-      __syncthreads();   // one per token: the next token writes the other half of `part`
-      if (threadIdx.x < a.K) {
-        float sum = 0.f;
-        if (pair.row >= 0)
-          for (int w = 0; w < W; ++w) sum += part[par][w][threadIdx.x];
-        a.dweight[static_cast<int64_t>(t) * a.K + threadIdx.x] = sum;
-      }
-      par ^= 1;
+      store_raw8<T, true>(static_cast<T*>(a.out) + static_cast<int64_t>(t) * a.H + c, a.H - c, lane, from_floats<T>(acc));
     }
   }
   cp_async_wait<0>();
 }
 
-template <typename T, int kRows, int kBatches, bool kBackward>
-cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
-  constexpr int kWarpBytes = kStages * (kRows + (kBackward ? 1 : 0)) * kSlice * static_cast<int>(sizeof(T));
-  auto* kernel = combine_pipe_kernel<T, kRows, kBatches, kBackward>;
-  // the warps that share the slices evenly, and blocks for about kPipeWarps warps on each SM
-  const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kPipeWarps<T, kBackward> - 1) / kPipeWarps<T, kBackward>;
-  const int warps = (slices + steps - 1) / steps;
-  const int target = kPipeWarps<T, kBackward> * 8 / kRows, per_sm = std::max(1, (target + warps / 2) / warps);
-  // allowed once per device; a second thread that gets here first does the same again
-  static std::atomic<uint64_t> allowed{0};
+// Backward.  One block of up to seven warps per token, in token order, and not blocks
+// that stay: what it stores, K rows for one, then fills the experts' segments in
+// address order (as in scatter_rows_kernel).  The blocks of an SM overlap each other;
+// a warp with several steps issues the next before it sums one.  The first blocks
+// zero the rows without a pair.  Measured (K = 8, bf16; 4096 tokens of 7168 columns,
+// 16384 of 2048): 162 and 180 us = 6.2 and 6.3 TB/s, against 171 and 205 us for
+// blocks that stay and 202 and 239 us with the rows loaded to registers; 14 warps and
+// one stage: 174 and 193 us.
+constexpr int kBackwardStages = 2;
+constexpr int kBackwardWarps = 7;
+
+template <typename T, int kRows, int kBatches>
+__global__ void __launch_bounds__(kBackwardWarps * 32)
+    combine_backward_pipe_kernel(const CombineArgs a, int stages, unsigned zero_blocks) {
+  constexpr int kStages = kBackwardStages;
+  constexpr int kStep = (kRows + 1) * kHalves<T>;            // the last slot row: the output's gradient
+  extern __shared__ __align__(16) uint4 pipe_smem[];
+  __shared__ float part[kBackwardWarps][kRows * kBatches];
+  T* drows = static_cast<T*>(a.out);
+  if (blockIdx.x < zero_blocks) {
+    zero_rows<T, true>(a.row_pair, static_cast<int64_t>(a.T) * a.K, blockIdx.x, zero_blocks, a.R, a.H, drows);
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+  const uint4* mine = pipe_smem + static_cast<size_t>(warp) * stages * kStep * 32 + lane;   // stages in use
+  const uint32_t mine_s = smem_u32(mine);
+  const T* rows = static_cast<const T*>(a.rows);
+  const int64_t t = blockIdx.x - zero_blocks;
+  const T* dout = static_cast<const T*>(a.dout) + t * a.H;
+  const int slices = (a.H + kSlice - 1) / kSlice;
+  const PairLane pair = load_pair(a.pair_row, a.weight, t, a.K, a.R, lane);
+  const int out_row = drows ? pair.row : -1;   // where this lane's pair is stored
+
+  int is = warp, ib = 0;
+  auto issue = [&](int stage) {
+    if (is < slices) {
+      const uint32_t dst = mine_s + stage * kStep * 512;
+      slot_copy<T>(dst + kRows * kHalves<T> * 512, dout, dout, is * kSlice, a.H, lane);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int row = __shfl_sync(0xffffffffu, pair.row, ib * kRows + j);
+        slot_copy<T>(dst + j * kHalves<T> * 512, row >= 0 ? rows + static_cast<int64_t>(row) * a.stride : nullptr, dout,
+                     is * kSlice, a.H, lane);
+      }
+      if (++ib == kBatches) {
+        ib = 0;
+        is += W;
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+  int stage = 0;
+  float dot[kBatches][kRows] = {};
+  for (int sl = warp; sl < slices; sl += W) {
+    const int c = sl * kSlice, n = a.H - c;
+#pragma unroll
+    for (int b = 0; b < kBatches; ++b) {
+      issue(stage == 0 ? kStages - 1 : stage - 1);
+      cp_async_wait<kStages - 1>();
+      const uint4* slot = mine + stage * kStep * 32;
+      float g[8];
+      to_floats(slot_load<T>(slot + kRows * kHalves<T> * 32), g);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int row = __shfl_sync(0xffffffffu, out_row, b * kRows + j);
+        const float w = __shfl_sync(0xffffffffu, pair.w, b * kRows + j);
+        float f[8];
+        to_floats(slot_load<T>(slot + j * kHalves<T> * 32), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot[b][j] = fmaf(g[i], f[i], dot[b][j]);
+        if (row >= 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = w * g[i];
+          store_raw8<T, true>(drows + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
+        }
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < kBatches; ++b)
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      float d = dot[b][j];
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+      if (lane == 0) part[warp][b * kRows + j] = d;
+    }
+  cp_async_wait<0>();
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < a.K) {
+    float sum = 0.f;
+    if (pair.row >= 0)   // lane k of warp 0 holds pair k
+      for (int w = 0; w < W; ++w) sum += part[w][threadIdx.x];
+    a.dweight[t * a.K + threadIdx.x] = sum;
+  }
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device; `allowed` remembers the devices
+// (a second thread that gets here first does the same again).
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& allowed) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const uint64_t bit = uint64_t{1} << (dev & 63);
-  if (dev >= 64 || !(allowed.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarpBytes * kPipeWarps<T, kBackward>);
-    if (e != cudaSuccess) return e;
-    allowed.fetch_or(bit, std::memory_order_release);
-  }
-  const int grid = std::min(a.T, sms * per_sm);
+  if (dev < 64 && (allowed.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+// The warps, at most `most`, that share a row's slices evenly.
+inline int warps_for(int H, int most) {
+  const int slices = (H + kSlice - 1) / kSlice, steps = (slices + most - 1) / most;
+  return (slices + steps - 1) / steps;
+}
+
+template <typename T, int kRows, int kBatches>
+cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
+  constexpr int kWarps = kForwardWarps<T>, kWarpBytes = kForwardStages * kRows * kHalves<T> * 512;
+  static std::atomic<uint64_t> allowed{0};
+  auto* kernel = combine_pipe_kernel<T, kRows, kBatches>;
+  const cudaError_t e = allow_smem(kernel, kWarpBytes * kWarps, allowed);
+  if (e != cudaSuccess) return e;
+  // blocks for about kWarps warps of eight rows on each SM
+  const int warps = warps_for(a.H, kWarps), target = kWarps * 8 / kRows;
+  const int grid = std::min(a.T, sms * std::max(1, (target + warps / 2) / warps));
   kernel<<<grid, warps * 32, kWarpBytes * warps, s>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T, bool kBackward>
-cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
-  if (a.K <= 2) return launch_pipe<T, 2, 1, kBackward>(a, sms, s);
-  if (a.K <= 4) return launch_pipe<T, 4, 1, kBackward>(a, sms, s);
-  if (a.K <= 8) return launch_pipe<T, 8, 1, kBackward>(a, sms, s);
-  return launch_pipe<T, 8, 2, kBackward>(a, sms, s);
+template <typename T, int kRows, int kBatches>
+cudaError_t launch_backward_pipe(const CombineArgs& a, cudaStream_t s) {
+  constexpr int kStageBytes = (kRows + 1) * kHalves<T> * 512;
+  static std::atomic<uint64_t> allowed{0};
+  auto* kernel = combine_backward_pipe_kernel<T, kRows, kBatches>;
+  const cudaError_t e = allow_smem(kernel, kStageBytes * kBackwardStages * kBackwardWarps, allowed);
+  if (e != cudaSuccess) return e;
+  // a warp with a single step uses one stage: more blocks fit an SM
+  const int warps = warps_for(a.H, kBackwardWarps), slices = (a.H + kSlice - 1) / kSlice;
+  const int stages = slices * kBatches <= warps ? 1 : kBackwardStages;
+  const unsigned zero_blocks = a.out ? zero_blocks_for(a.R) : 0u;
+  kernel<<<zero_blocks + a.T, warps * 32, kStageBytes * stages * warps, s>>>(a, stages, zero_blocks);
+  return cudaGetLastError();
 }
 
-// ---- the plain form, for rows of any alignment (and fp32 backward) ----
+template <typename T>
+cudaError_t launch_pipe(const CombineArgs& a, int sms, cudaStream_t s) {
+  if (a.K <= 2) return launch_pipe<T, 2, 1>(a, sms, s);
+  if (a.K <= 4) return launch_pipe<T, 4, 1>(a, sms, s);
+  if (a.K <= 8) return launch_pipe<T, 8, 1>(a, sms, s);
+  return launch_pipe<T, 8, 2>(a, sms, s);
+}
+
+template <typename T>
+cudaError_t launch_backward_pipe(const CombineArgs& a, cudaStream_t s) {
+  if (a.K <= 2) return launch_backward_pipe<T, 2, 1>(a, s);
+  if (a.K <= 4) return launch_backward_pipe<T, 4, 1>(a, s);
+  if (a.K <= 8) return launch_backward_pipe<T, 8, 1>(a, s);
+  return launch_backward_pipe<T, 8, 2>(a, s);
+}
+
+// ---- the plain form, for rows of any alignment ----
 
 inline unsigned blocks(int64_t items, int per) { return static_cast<unsigned>((items + per - 1) / per); }
 
@@ -711,14 +799,14 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const CombineAr
 
 // `warps` warps per token share its slices, `tokens` tokens per block.  The first
 // blocks zero the rows without a pair.
-template <typename T, bool kVec>
+template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(const CombineArgs a, int warps, int tokens,
                                                                           unsigned zero_blocks) {
   const T* rows = static_cast<const T*>(a.rows);
   const T* dout = static_cast<const T*>(a.dout);
   T* drows = static_cast<T*>(a.out);
   if (blockIdx.x < zero_blocks) {
-    zero_rows<T, kVec>(a.row_pair, static_cast<int64_t>(a.T) * a.K, blockIdx.x, zero_blocks, a.R, a.H, drows);
+    zero_rows<T, false>(a.row_pair, static_cast<int64_t>(a.T) * a.K, blockIdx.x, zero_blocks, a.R, a.H, drows);
     return;
   }
   __shared__ float part[kRowWarps][KF_SORT_MAX_TOP_K];
@@ -733,11 +821,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(const 
     for (int c = w0 * kSlice; live && c < a.H; c += warps * kSlice) {
       const int n = a.H - c;
       Raw8<T> v[kBatch<T>];
-      const Raw8<T> graw = load_raw8<T, kVec>(dout + t * a.H + c, n, lane);
+      const Raw8<T> graw = load_raw8<T, false>(dout + t * a.H + c, n, lane);
 #pragma unroll
       for (int j = 0; j < kBatch<T>; ++j) {
         const int row = __shfl_sync(0xffffffffu, mine.row, k0 + j);
-        v[j] = load_raw8<T, kVec>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * a.stride + c, row < 0 ? 0 : n, lane);
+        v[j] = load_raw8<T, false>(rows + static_cast<int64_t>(row < 0 ? 0 : row) * a.stride + c, row < 0 ? 0 : n, lane);
       }
       float g[8];
       to_floats(graw, g);
@@ -752,7 +840,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(const 
         if (drows && row >= 0) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = w * g[i];
-          store_raw8<T, kVec>(drows + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
+          store_raw8<T, false>(drows + static_cast<int64_t>(row) * a.H + c, n, lane, from_floats<T>(f));
         }
       }
     }
@@ -779,13 +867,13 @@ cudaError_t launch_combine(const CombineArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename T, bool kVec>
+template <typename T>
 cudaError_t launch_combine_backward(const CombineArgs& a, cudaStream_t s) {
   // as many warps as share the slices evenly, kRowWarps at most
   const int slices = (a.H + kSlice - 1) / kSlice, steps = (slices + kRowWarps - 1) / kRowWarps;
   const int warps = (slices + steps - 1) / steps, tokens = kRowWarps / warps;
   const unsigned zero_blocks = a.out ? zero_blocks_for(a.R) : 0u;
-  combine_backward_kernel<T, kVec>
+  combine_backward_kernel<T>
       <<<zero_blocks + blocks(a.T, tokens), warps * tokens * 32, 0, s>>>(a, warps, tokens, zero_blocks);
   return cudaGetLastError();
 }
@@ -912,7 +1000,7 @@ int kf_combine_tokens(const void* rows, int32_t dtype, int64_t rows_stride, int3
     using E = ElemOf<decltype(t)>;
     constexpr bool kVec = decltype(v)::value;
     if constexpr (kVec)
-      return launch_pipe<E, false>(a, sms, s);
+      return launch_pipe<E>(a, sms, s);
     else
       return launch_combine<E>(a, s);
   }));
@@ -946,12 +1034,10 @@ int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype
       return launch_scatter<E, kVec, true>(grad_output, width, pair_row, row_pair, topk_weight, num_tokens, top_k, width,
                                            num_rows, grad_rows, false, s);
     const CombineArgs a{rows, grad_output, pair_row, row_pair, topk_weight, grad_rows, grad_weight, rows_stride, num_tokens, top_k, width, num_rows};
-    // fp32 takes the plain form: its steps are twice as long, and what it stores covers long runs
-    // as it is (4096 tokens, K = 8, 28672-byte rows: 323 us against 368 us; K = 4: 168 us against 181 us)
-    if constexpr (kVec && sizeof(E) == 2)
-      return launch_pipe<E, true>(a, sms, s);
+    if constexpr (kVec)
+      return launch_backward_pipe<E>(a, s);
     else
-      return launch_combine_backward<E, kVec>(a, s);
+      return launch_combine_backward<E>(a, s);
   }));
 }
 
