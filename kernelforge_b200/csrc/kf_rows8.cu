@@ -259,6 +259,8 @@ __device__ __forceinline__ Unit unit_of(int slices) {
 // most an eighth of the warps half empty, else one.
 inline bool pairs_of_slices(int slices) { return slices % 2 == 0 || slices >= 7; }
 
+// Bound by issuing its instructions as much as by memory: 19 us = 4.6 TB/s for 4096 rows
+// of 7168 bf16 columns, 12.7 us = 5.8 TB/s for 2048 of fp32.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t stride, int R, int W,
                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
@@ -295,7 +297,7 @@ __device__ __forceinline__ Raw8<T> restored(uint2 codes, const float (&s)[2]) {
   return from_floats<T>(v);
 }
 
-// Rows as they were.
+// Rows as they were.  12.8 us = 6.9 TB/s for 4096 rows of 7168 bf16 columns.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __restrict__ codes,
                                                             const uint8_t* __restrict__ exps, int R, int W,
@@ -322,6 +324,8 @@ __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __res
 // Rows in expert order: a block holds a token's row across its warps, two slices
 // each, decodes it once and stores it K times (as scatter_rows_kernel, whose reason
 // for one block per token holds here too).  The first blocks zero the rows of no pair.
+// 93 us = 5.9 TB/s for 4096 tokens of 7168 bf16 columns into 36608 rows; a warp per
+// output row, which decodes a row K times, took 214 us.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int T_, int W,
@@ -363,6 +367,8 @@ __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
 }
 
 // h = [up | gate]: act = up * silu(gate), and h kept in 8 bits (each half's blocks begin at its own column 0).
+// 97 us = 5.5 TB/s for 32768 rows of 2048 bf16 columns each (bound by issue and memory alike: 140 us with divisions
+// and a check per element); fp32 rows 6.8 TB/s.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restrict__ h, int64_t stride, int R, int I,
                                                                 T* __restrict__ act, uint8_t* __restrict__ codes,
@@ -405,6 +411,8 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
 }
 
 // From the kept values u, g and d = dL/dact: du = d g s, dg = d u (s + g s (1 - s)), act = u g s, with s = sigmoid(g).
+// One pass: 102 us = 6.6 TB/s for 32768 rows of 2048 bf16 columns, bound by memory (133 us before its sigmoid took 4
+// instructions).
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ exps,

@@ -1,13 +1,16 @@
 // Tokens sorted by expert and back, for rows of bf16, fp16 or fp32.
 //
-//   order    a stable counting sort of the (token, choice) pairs by local expert:
-//            per-chunk histograms, one scan over chunks and experts, and each
-//            pair's row = its expert's segment start + its pairs in earlier chunks
-//            + its pairs earlier in the chunk
-//   gather   rows[r] = x[token of row_pair[r]], zeros for a row without a pair
-//   combine  out[t] = sum_k w[t,k] rows[pair_row[t,k]], k ascending, fp32, one
-//            rounding; without weights it is the gradient of the gather
-//   combine_backward  drows[r] = w[p] dout[t], dw[t,k] = <dout[t], rows[pair_row[t,k]]>
+//   order     a stable counting sort of the (token, choice) pairs by local expert:
+//             a pair's row = its expert's segment start + the expert's pairs before it
+//   scatter   rows[pair_row[t,k]] = x[t], zeros in the rows of no pair
+//   combine   out[t] = sum_k w[t,k] rows[pair_row[t,k]], k ascending, fp32, one
+//             rounding; without weights it is the gradient of the sort
+//   backward  drows[r] = w[p] dout[t], dw[t,k] = <dout[t], rows[pair_row[t,k]]>
+//
+// A sort is one launch when it is small, else placing (after a histogram, for many
+// pairs) and the scatter, chained by programmatic launches.  All of it but the order
+// (some 9 us at 32768 pairs, of them 3 us histogram) is bound by memory: every row is
+// read or written once, at 5.6 to 6.6 TB/s where a plain copy reaches 6.55.
 //
 // The reference sorts and combines inside its kernel() only, for its own FP8
 // layer and without gradients (solution/triton/kernel.py:46-82, :1920-1925).
@@ -44,7 +47,7 @@ inline OrderPlan plan_order(int T, int K) {
   return OrderPlan{ct, (T + ct - 1) / ct};
 }
 
-// hist[c][e] = pairs of local expert e among the tokens of chunk c.
+// hist[c][e] = pairs of local expert e among the tokens of chunk c.  2.7 us at 32768 or 131072 pairs.
 __global__ void __launch_bounds__(kHistThreads) order_hist_kernel(const int32_t* __restrict__ ids, int n, int E,
                                                                   int offset, int chunk_pairs,
                                                                   int32_t* __restrict__ hist) {
@@ -90,6 +93,8 @@ struct PlaceArgs {
 // Ranks.  A pair's row is its expert's next row, plus the pairs of its expert in
 // the block's earlier warps, plus those in lower lanes of its own warp: stable and
 // without atomics on the order.
+// Bound by latencies (ids, histogram, some ten block barriers): 6.2 us at 32768 pairs
+// and 6.7 us at 131072, waiting for the histogram included.
 __global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const PlaceArgs a) {
   grid_dep_trigger();
   __shared__ int32_t total[kEG], before[kEG];        // before becomes the next row of each expert
@@ -227,7 +232,10 @@ __global__ void __launch_bounds__(kPlaceThreads, 1) place_tokens_kernel(const Pl
 // Small calls (at most kSmallPairs pairs, few rows) in one launch.  Every block
 // ranks all pairs -- a call's worth of ids is a few loads per thread -- and then
 // copies its share of the (token, slice) units and zeroes its share of the rows
-// without a pair; a warp's first unit is on its way from memory meanwhile.
+// without a pair; a warp's first unit is on its way from memory meanwhile.  With K = 8
+// and bf16, against placing and scatter: 3.1 us against 6.4 us for one token of 7168
+// columns, 3.4 against 7.0 for 16, 7.6 against 10.8 for 128, and 4.7 against 5.8 for
+// 128 tokens of 64 columns.
 constexpr int kSmallThreads = 256;
 constexpr int kSmallPairs = 1024;
 
@@ -767,6 +775,8 @@ template <typename T>
 constexpr int kBatch = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight together
 
 // One warp per (token, slice of 256 columns), consecutive warps on consecutive slices.
+// 25 us = 3.1 TB/s for 4096 tokens of 1031 columns, K = 8, bf16 (rows between two words:
+// bound by the shuffles), 21 us for 1030 columns.
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const CombineArgs a) {
   const T* rows = static_cast<const T*>(a.rows);
@@ -798,7 +808,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const CombineAr
 }
 
 // `warps` warps per token share its slices, `tokens` tokens per block.  The first
-// blocks zero the rows without a pair.
+// blocks zero the rows without a pair.  64 us = 2.4 TB/s at the sizes above, 45 us for
+// 1030 columns; with one element per access it took 165 us.
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(const CombineArgs a, int warps, int tokens,
                                                                           unsigned zero_blocks) {
@@ -885,7 +896,8 @@ bool valid_shape(int32_t T, int32_t K, int64_t H, int32_t dtype) {
 // Rows of a type begin at a multiple of its size (a null pointer does).
 bool elem_aligned(const void* p, int32_t dtype) { return reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype) == 0; }
 
-// Small calls whose rows are at most this many bytes in all are sorted in one launch.
+// Small calls (kSmallPairs) whose rows are at most this many bytes in all are sorted in
+// one launch: above it the bandwidth of the scatter is worth the launch.
 constexpr int64_t kSmallBytes = 16 << 20;
 
 template <typename P>
