@@ -71,23 +71,21 @@ Tensor new_tensor(at::IntArrayRef shape, at::ScalarType dtype, const at::Device&
   return Tensor(at::detail::empty_cuda(shape, dtype, dev, std::nullopt));
 }
 
-// Whether a call on `t` is recorded for autograd.  During a stream capture a leaf whose
-// gradient accumulator already lives on another stream -- an eager graph of the same
-// leaf is still alive -- is refused: the backward pass would make that stream wait for
-// the capturing one, which invalidates the capture inside the autograd engine.
-bool wants_grad(const Tensor& t) {
-  if (!at::GradMode::is_enabled() || !t.requires_grad()) return false;
-  if (t.is_leaf()) {
-    const at::cuda::CUDAStream now = at::cuda::getCurrentCUDAStream(t.device().index());
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(now.stream(), &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
-      const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
-      TORCH_CHECK(!acc || !acc->stream().has_value() || *acc->stream() == now.unwrap(),
-                  "a captured call on a leaf tensor whose eager autograd graph is still alive: release that graph "
-                  "first, or capture a detached copy that requires grad");
-    }
-  }
-  return true;
+bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// During a stream capture a leaf whose gradient accumulator already lives on another
+// stream -- an eager graph of the same leaf is still alive -- is refused: the backward
+// pass would make that stream wait for the capturing one, which invalidates the capture
+// inside the autograd engine.  `t`: an argument as the caller gave it.
+void refuse_shared_leaf(const Tensor& t) {
+  if (!t.defined() || !t.is_cuda() || !t.is_leaf() || !wants_grad(t)) return;
+  const at::cuda::CUDAStream now = at::cuda::getCurrentCUDAStream(t.device().index());
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(now.stream(), &cap) != cudaSuccess || cap == cudaStreamCaptureStatusNone) return;
+  const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
+  TORCH_CHECK(!acc || !acc->stream().has_value() || *acc->stream() == now.unwrap(),
+              "a captured call on a leaf tensor whose eager autograd graph is still alive: release that graph first, "
+              "or capture a detached copy that requires grad");
 }
 
 void refuse_double_backward(const char* what) {
@@ -192,6 +190,7 @@ struct SortFn : public torch::autograd::Function<SortFn> {
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> sort_tokens(const Tensor& x_in, const Tensor& topk_idx,
                                                                int64_t num_experts, int64_t expert_offset,
                                                                int64_t row_align, std::optional<int64_t> max_rows) {
+  refuse_shared_leaf(x_in);
   const Tensor x = expect_rows(x_in, "x");
   const int64_t T = x.size(0);
   TORCH_CHECK(topk_idx.dim() == 2 && topk_idx.size(0) == T && topk_idx.size(1) >= 1 &&
@@ -255,6 +254,8 @@ Tensor expect_weight(const std::optional<Tensor>& w, const Order& o, const at::D
 
 Tensor combine_tokens(const Tensor& rows_in, const Tensor& pair_row, const Tensor& row_pair,
                       const std::optional<Tensor>& topk_weight) {
+  refuse_shared_leaf(rows_in);
+  if (topk_weight.has_value()) refuse_shared_leaf(*topk_weight);
   const Tensor rows = expect_rows(rows_in, "rows");
   const Order o = expect_order(pair_row, row_pair, rows.device());
   TORCH_CHECK(rows.size(0) == o.row_pair.size(0), "rows has ", rows.size(0), " rows, the order ", o.row_pair.size(0));
@@ -332,6 +333,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 };
 
 std::tuple<Tensor, Tensor> route(const Tensor& routing_logits, const Tensor& routing_bias, double rsf) {
+  refuse_shared_leaf(routing_logits);
   check_cuda(routing_logits, "routing_logits");
   const at::Device dev = routing_logits.device();
   TORCH_CHECK(routing_logits.dim() == 2, "routing_logits must be [T, 256]");
@@ -448,6 +450,7 @@ struct SwigluFn : public torch::autograd::Function<SwigluFn> {
 };
 
 Tensor swiglu(const Tensor& h) {
+  refuse_shared_leaf(h);
   if (wants_grad(h)) return SwigluFn::apply(h);
   return std::get<0>(swiglu_forward(h, false));
 }

@@ -76,7 +76,7 @@ def sort_tokens(x: torch.Tensor, topk_idx: torch.Tensor, num_experts: int, exper
     ``x`` ``[T, H]``, ``topk_idx`` int32 ``[T, K]`` with global expert ids, K from 1 to 16.  The local
     experts are ``[expert_offset, expert_offset + num_experts)`` within the layer's 256; a pair with
     any other id (such as -1 for a masked token) gets no row.  Each expert's rows are in (token,
-    choice) order and start at a multiple of ``row_align``; rows that belong to no pair are zero.
+    choice) order and start at a multiple of ``row_align`` (1 to 1024); rows that belong to no pair are zero.
 
     ``R`` is what the worst routing needs, ``T * K + min(T * K, num_experts) * (row_align - 1)`` cut to a
     multiple of ``row_align``, or ``max_rows`` (a multiple of it): then pairs whose row would lie past

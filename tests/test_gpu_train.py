@@ -263,7 +263,8 @@ def test_rows_in_8_bits_at_the_ends(w, dtype):
     info = torch.finfo(dtype)
     rows = [torch.zeros(w), torch.full((w,), info.max), torch.full((w,), -info.max), torch.full((w,), info.tiny),
             torch.linspace(-1, 1, w) * info.max, torch.linspace(-448, 448, w), torch.linspace(-1, 1, w) * 449,
-            torch.linspace(-17.5, 17.5, w), 2.0 ** torch.linspace(-24, 15, w), torch.linspace(0, 2.0 ** -9, w)]
+            torch.linspace(-17.5, 17.5, w), 2.0 ** torch.linspace(-24, 15, w), torch.linspace(0, 2.0 ** -9, w),
+            torch.linspace(-1, 1, w) * info.tiny, torch.linspace(0, 1, w) * info.tiny / 4]
     odd = torch.linspace(-3, 3, w)
     odd[5], odd[7], odd[w - 1] = float("inf"), float("nan"), float("-inf")
     rows += [odd, torch.full((w,), float("nan")), torch.full((w,), float("inf"))]
@@ -508,7 +509,13 @@ def test_capture_with_an_eager_graph_of_the_same_leaf_is_refused():
     eager, order = train.sort_tokens(x, ids, 4)        # alive, on the default stream
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
-    for call in (lambda: train.sort_tokens(x, ids, 4), lambda: train.swiglu(x), lambda: train.combine_tokens(x, order)):
+    w = torch.ones(8, 1, device="cuda", requires_grad=True)
+    also = train.combine_tokens(eager.detach(), order, w)
+    logits = torch.randn(8, 256, device="cuda", requires_grad=True)
+    bias = torch.zeros(256, dtype=torch.bfloat16, device="cuda")
+    fourth = train.route(logits, bias, 1.0)
+    for call in (lambda: train.sort_tokens(x, ids, 4), lambda: train.swiglu(x), lambda: train.combine_tokens(x, order),
+                 lambda: train.combine_tokens(eager.detach(), order, w), lambda: train.route(logits, bias, 1.0)):
         gr = torch.cuda.CUDAGraph()
         with torch.cuda.stream(side):
             gr.capture_begin()
@@ -519,7 +526,7 @@ def test_capture_with_an_eager_graph_of_the_same_leaf_is_refused():
                 gr.capture_end()
     torch.cuda.synchronize()
     dx, = torch.autograd.grad(eager, x, torch.ones_like(eager))
-    assert (dx == 1).all()
+    assert (dx == 1).all() and also.requires_grad and fourth[1].requires_grad
 
 
 def test_two_streams_at_once():

@@ -109,7 +109,7 @@ def _sort(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(T=(1 << 24) + 1), dict(K=0), dict(K=17), dict(H=0), dict(H=(1 << 20) + 1),
-                                 dict(E=0), dict(E=257), dict(off=-1), dict(off=249), dict(align=0), dict(align=1025),
+                                 dict(E=0), dict(E=257), dict(off=-1), dict(off=249), dict(off=2 ** 31 - 1), dict(align=0), dict(align=1025),
                                  dict(align=16, R=24), dict(R=-1), dict(R=(1 << 30) + 1), dict(dtype=3), dict(dtype=-1), dict(stride=-1),
                                  dict(x=NULL), dict(x=vp(257)), dict(rows=vp(258), dtype=2), dict(ids=NULL), dict(rows=NULL), dict(pr=NULL), dict(rp=NULL),
                                  dict(cnt=NULL), dict(st=NULL), dict(T=65536, R=65536 * 2, ws=NULL)])
