@@ -24,17 +24,20 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
+// Exponents are held as they are stored, e + 127 (1 .. 247).
 template <typename T>
-constexpr int kTopExponent = 120;   // 256 * 2^120 = 2^128 is beyond bf16 and fp32
+constexpr int kTopExponent = 127 + 120;   // 256 * 2^120 = 2^128 is beyond bf16 and fp32
 template <>
-constexpr int kTopExponent<__half> = 8;   // 256 * 2^8 = 65536 is beyond fp16
+constexpr int kTopExponent<__half> = 127 + 8;   // 256 * 2^8 = 65536 is beyond fp16
 
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+__device__ __forceinline__ float scale_of(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }   // 2^(e - 127)
+__device__ __forceinline__ float inverse_scale(int e) { return scale_of(254 - e); }
 
-// Smallest e >= -126 with amax <= 448 * 2^e = 1.75 * 2^(e+8), amax finite and not negative.
+// Smallest e >= 1 with amax <= 448 * 2^(e - 127) = 1.75 * 2^(e - 119), amax finite and not
+// negative: its exponent field less 8, and one more where the mantissa is above 1.75,
+// which adding 2^23 - 1 - 0.75 * 2^23 carries into the field.
 __device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
-  const int e = static_cast<int>(amax_bits >> 23) - 135 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < -126 ? -126 : e;
+  return max(static_cast<int>((amax_bits + 0x1fffffu) >> 23) - 8, 1);
 }
 
 // Magnitudes as keys in the type's own bits: larger magnitude, larger key.  Above
@@ -56,13 +59,18 @@ __device__ __forceinline__ uint32_t key_bits(uint32_t key, const __half*) {
 }
 
 __device__ __forceinline__ uint32_t max2_keys(uint32_t a, uint32_t b, const __nv_bfloat16*) {
-  const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)),
-                                       __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 __device__ __forceinline__ uint32_t max2_keys(uint32_t a, uint32_t b, const __half*) {
-  const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+  const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&m);
+}
+
+// The larger magnitudes of words i and i + 1 of a lane's 16-bit elements.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_keys(const Raw8<T>& r, int i) {
+  return max2_keys(r.x[i] & 0x7fff7fffu, r.x[i + 1] & 0x7fff7fffu, static_cast<const T*>(nullptr));
 }
 
 // A slice of 256 columns = two blocks.  The vector form of 16-bit types has a block
@@ -80,14 +88,14 @@ __device__ __forceinline__ void block_keys(const Raw8<T>& r, uint32_t (&key)[2])
       key[h] = __reduce_max_sync(0xffffffffu, max(max(r.x[4 * h] & 0x7fffffffu, r.x[4 * h + 1] & 0x7fffffffu),
                                                   max(r.x[4 * h + 2] & 0x7fffffffu, r.x[4 * h + 3] & 0x7fffffffu)));
   } else if constexpr (kHalfWarp<T, kVec>) {
-    uint32_t m = max2_keys(max2_keys(r.x[0], r.x[1], type), max2_keys(r.x[2], r.x[3], type), type);
+    uint32_t m = max2_keys(pair_keys(r, 0), pair_keys(r, 2), type);
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) m = max2_keys(m, __shfl_xor_sync(0xffffffffu, m, off), type);
     key[0] = key[1] = max(m & 0xffffu, m >> 16);
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t m = max2_keys(r.x[2 * h], r.x[2 * h + 1], type);
+      const uint32_t m = pair_keys(r, 2 * h);
       key[h] = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
     }
   }
@@ -98,8 +106,8 @@ template <typename T, bool kVec>
 __device__ __forceinline__ void block_keys2(const Raw8<T>& a, const Raw8<T>& b, uint32_t (&ka)[2], uint32_t (&kb)[2]) {
   if constexpr (kHalfWarp<T, kVec>) {
     const T* type = nullptr;
-    const uint32_t ma = max2_keys(max2_keys(a.x[0], a.x[1], type), max2_keys(a.x[2], a.x[3], type), type);
-    const uint32_t mb = max2_keys(max2_keys(b.x[0], b.x[1], type), max2_keys(b.x[2], b.x[3], type), type);
+    const uint32_t ma = max2_keys(pair_keys(a, 0), pair_keys(a, 2), type);
+    const uint32_t mb = max2_keys(pair_keys(b, 0), pair_keys(b, 2), type);
     uint32_t m = max2_keys(__byte_perm(ma, mb, 0x5410), __byte_perm(ma, mb, 0x7632), type);
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) m = max2_keys(m, __shfl_xor_sync(0xffffffffu, m, off), type);
@@ -136,7 +144,7 @@ __device__ __noinline__ void rare_blocks(float (&q)[8], int (&e)[2]) {
   for (int j = 0; j < 8; ++j) {
     const float v = q[j];
     const float limit = e[j >> 2] == kTopExponent<T> ? 240.f : 448.f;
-    q[j] = fminf(fmaxf(v * pow2(-e[j >> 2]), -limit), limit);
+    q[j] = fminf(fmaxf(v * inverse_scale(e[j >> 2]), -limit), limit);
     if ((__float_as_uint(v) & 0x7fffffffu) >= 0x7f800000u) q[j] = __uint_as_float(0x7fffffffu);
   }
 }
@@ -153,7 +161,7 @@ __device__ __forceinline__ uint2 encode8(const float (&v)[8], const uint32_t (&k
   } else {
     e[0] = block_exponent(key_bits(key[0], type));
     e[1] = kHalfWarp<T, kVec> ? e[0] : block_exponent(key_bits(key[1], type));
-    const float inv[2] = {pow2(-e[0]), pow2(-e[1])};
+    const float inv[2] = {inverse_scale(e[0]), inverse_scale(e[1])};
 #pragma unroll
     for (int j = 0; j < 8; ++j) q[j] = v[j] * inv[j >> 2];
   }
@@ -196,9 +204,9 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* __restrict__ slice, i
 template <typename T, bool kVec>
 __device__ __forceinline__ void store_exponents(uint8_t* __restrict__ exps, int n, int lane, const int (&e)[2]) {
   if (kHalfWarp<T, kVec>) {
-    if ((lane & 15) == 0 && (lane >> 4) * kBlk < n) exps[lane >> 4] = static_cast<uint8_t>(e[0] + 127);
+    if ((lane & 15) == 0 && (lane >> 4) * kBlk < n) exps[lane >> 4] = static_cast<uint8_t>(e[0]);
   } else {
-    if (lane < 2 && lane * kBlk < n) exps[lane] = static_cast<uint8_t>((lane ? e[1] : e[0]) + 127);
+    if (lane < 2 && lane * kBlk < n) exps[lane] = static_cast<uint8_t>(lane ? e[1] : e[0]);
   }
 }
 
@@ -207,10 +215,10 @@ template <typename T, bool kVec>
 __device__ __forceinline__ void load_scales(const uint8_t* __restrict__ exps, int n, int lane, float (&s)[2]) {
   if (kHalfWarp<T, kVec>) {
     const int b = lane >> 4;
-    s[0] = s[1] = b * kBlk < n ? __uint_as_float(static_cast<uint32_t>(__ldg(exps + b)) << 23) : 0.f;
+    s[0] = s[1] = b * kBlk < n ? scale_of(__ldg(exps + b)) : 0.f;
   } else {
-    s[0] = 0 < n ? __uint_as_float(static_cast<uint32_t>(__ldg(exps)) << 23) : 0.f;
-    s[1] = kBlk < n ? __uint_as_float(static_cast<uint32_t>(__ldg(exps + 1)) << 23) : 0.f;
+    s[0] = 0 < n ? scale_of(__ldg(exps)) : 0.f;
+    s[1] = kBlk < n ? scale_of(__ldg(exps + 1)) : 0.f;
   }
 }
 
@@ -242,17 +250,32 @@ __device__ __forceinline__ float sigmoid(float x) {
   }
 }
 
+// Division of n < 2^31 by a constant of the launch, 1 <= d <= 4096, as a product: with
+// 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d) the error of n m / 2^(31+s) is below
+// n / 2^(31+s) < 2^-s <= 1 / d, too little to reach the next integer.
+struct Divisor {
+  uint32_t m, shift;
+};
+inline Divisor divisor_of(uint32_t d) {
+  uint32_t s = 0;
+  while ((1u << s) < d) ++s;
+  return s == 0 ? Divisor{0u, 0u}   // d = 1
+                : Divisor{static_cast<uint32_t>(((uint64_t{1} << (31 + s)) + d - 1) / d), s - 1};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) { return d.m ? __umulhi(n, d.m) >> d.shift : n; }
+
 // One warp per (row, group of kGroup slices), consecutive warps on consecutive
-// groups of a row: this warp's row and first slice.
+// groups of a row: this warp's row and first slice.  `by`: the divisor for a row's groups.
 struct Unit {
   int64_t row;
   int slice;
 };
 template <int kGroup>
-__device__ __forceinline__ Unit unit_of(int slices) {
+__device__ __forceinline__ Unit unit_of(int slices, const Divisor& by) {
   const unsigned groups = (slices + kGroup - 1) / kGroup;
   const unsigned u = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  return Unit{u / groups, static_cast<int>(u % groups) * kGroup};
+  const unsigned row = divide(u, by);
+  return Unit{row, static_cast<int>(u - row * groups) * kGroup};
 }
 
 // Slices per warp whose loads are in flight together: two, where that leaves at
@@ -263,10 +286,11 @@ inline bool pairs_of_slices(int slices) { return slices % 2 == 0 || slices >= 7;
 // of 7168 bf16 columns, 12.7 us = 5.8 TB/s for 2048 of fp32.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t stride, int R, int W,
-                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
+                                                         const Divisor by, uint8_t* __restrict__ codes,
+                                                         uint8_t* __restrict__ exps) {
   const int lane = threadIdx.x & 31;
   const int slices = (W + kSlice - 1) / kSlice, nb = (W + kBlk - 1) / kBlk;
-  const Unit u = unit_of<kGroup>(slices);
+  const Unit u = unit_of<kGroup>(slices, by);
   if (u.row >= R) return;
   const T* src = x + u.row * stride;
   Raw8<T> raw[kGroup];
@@ -301,10 +325,10 @@ __device__ __forceinline__ Raw8<T> restored(uint2 codes, const float (&s)[2]) {
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __restrict__ codes,
                                                             const uint8_t* __restrict__ exps, int R, int W,
-                                                            T* __restrict__ out) {
+                                                            const Divisor by, T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   const int slices = (W + kSlice - 1) / kSlice, nb = (W + kBlk - 1) / kBlk;
-  const Unit u = unit_of<kGroup>(slices);
+  const Unit u = unit_of<kGroup>(slices, by);
   if (u.row >= R) return;
   uint2 q[kGroup];
   float s[kGroup][2];
@@ -371,11 +395,12 @@ __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
 // and a check per element); fp32 rows 6.8 TB/s.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restrict__ h, int64_t stride, int R, int I,
-                                                                T* __restrict__ act, uint8_t* __restrict__ codes,
+                                                                const Divisor by, T* __restrict__ act,
+                                                                uint8_t* __restrict__ codes,
                                                                 uint8_t* __restrict__ exps) {
   const int lane = threadIdx.x & 31;
   const int slices = (I + kSlice - 1) / kSlice, nb = (I + kBlk - 1) / kBlk;
-  const Unit unit = unit_of<kGroup>(slices);
+  const Unit unit = unit_of<kGroup>(slices, by);
   if (unit.row >= R) return;
   const int64_t r = unit.row;
   Raw8<T> ru[kGroup], rg[kGroup];
@@ -417,10 +442,11 @@ template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ exps,
                                                                     const T* __restrict__ grad, int64_t stride, int R,
-                                                                    int I, T* __restrict__ dh, T* __restrict__ act) {
+                                                                    int I, const Divisor by, T* __restrict__ dh,
+                                                                    T* __restrict__ act) {
   const int lane = threadIdx.x & 31;
   const int slices = (I + kSlice - 1) / kSlice, nb = (I + kBlk - 1) / kBlk;
-  const Unit unit = unit_of<kGroup>(slices);
+  const Unit unit = unit_of<kGroup>(slices, by);
   if (unit.row >= R) return;
   const int64_t r = unit.row;
   Raw8<T> rd[kGroup];
@@ -468,7 +494,7 @@ bool valid_rows(int64_t R, int64_t W, int32_t dtype) {
 unsigned grid_of(int64_t R, int64_t W) {
   const int64_t slices = (W + kSlice - 1) / kSlice, group = pairs_of_slices(static_cast<int>(slices)) ? 2 : 1;
   const int64_t units = R * ((slices + group - 1) / group);
-  return units <= 0xffffffffll - kWarps ? static_cast<unsigned>((units + kWarps - 1) / kWarps) : 0u;
+  return units <= 0x7fffffffll - kWarps ? static_cast<unsigned>((units + kWarps - 1) / kWarps) : 0u;
 }
 
 // `a`: a power of two; rows of a type begin at a multiple of its size
@@ -479,17 +505,18 @@ struct IntTag {
   static constexpr int value = N;
 };
 
-// Calls f(type, access form, group) for rows of `width` columns.
+// Calls f(type, access form, group, divisor for a row's groups) for rows of `width` columns.
 template <typename F>
 int launch(int32_t dtype, bool vec, int32_t width, F&& f) {
   int sms = 0;
   const int rc = device_ready(&sms);
   if (rc != KF_OK) return rc;
   return dispatch_rows(dtype, vec, [&](auto t, auto v) {
-           if (pairs_of_slices((width + kSlice - 1) / kSlice))
-             f(t, v, IntTag<2>{});
+           const int slices = (width + kSlice - 1) / kSlice;
+           if (pairs_of_slices(slices))
+             f(t, v, IntTag<2>{}, divisor_of((slices + 1) / 2));
            else
-             f(t, v, IntTag<1>{});
+             f(t, v, IntTag<1>{}, divisor_of(slices));
            return cudaGetLastError();
          }) == cudaSuccess
              ? KF_OK
@@ -513,10 +540,10 @@ int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, i
   const unsigned grid = grid_of(num_rows, width);
   if (!x || !codes || !exponents || !grid || !aligned(x, elem_bytes(dtype))) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(x, x_stride, width, dtype) && aligned(codes, 8);
-  return launch(dtype, vec, width, [&](auto t, auto v, auto g) {
+  return launch(dtype, vec, width, [&](auto t, auto v, auto g, const Divisor& by) {
     using E = ElemOf<decltype(t)>;
     pack8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const E*>(x), x_stride, num_rows, width, static_cast<uint8_t*>(codes),
+        static_cast<const E*>(x), x_stride, num_rows, width, by, static_cast<uint8_t*>(codes),
         static_cast<uint8_t*>(exponents));
   });
 }
@@ -534,7 +561,7 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
   const unsigned grid = grid_of(num_rows, width);
   if (!output || (num_rows > 0 && !grid) || !aligned(output, elem_bytes(dtype))) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(output, width, width, dtype) && aligned(codes, 8);
-  return launch(dtype, vec, width, [&](auto t, auto v, auto g) {
+  return launch(dtype, vec, width, [&](auto t, auto v, auto g, const Divisor& by) {
     using E = ElemOf<decltype(t)>;
     const uint8_t* c = static_cast<const uint8_t*>(codes);
     const uint8_t* e = static_cast<const uint8_t*>(exponents);
@@ -546,7 +573,8 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
           c, e, num_rows, width, pair_row, row_pair, top_k, out_rows, p.warps, p.tokens, zero_blocks,
           static_cast<E*>(output));
     } else {
-      restore8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, s>>>(c, e, num_rows, width, static_cast<E*>(output));
+      restore8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, s>>>(c, e, num_rows, width, by,
+                                                                                     static_cast<E*>(output));
     }
   });
 }
@@ -559,10 +587,10 @@ int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_
   if (!h || !act || !codes != !exponents || !grid) return KF_ERR_INVALID_ARGUMENT;
   if (!aligned(h, elem_bytes(dtype)) || !aligned(act, elem_bytes(dtype))) return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(h, h_stride, inter, dtype) && vec_rows(act, inter, inter, dtype) && aligned(codes, 8);
-  return launch(dtype, vec, inter, [&](auto t, auto v, auto g) {
+  return launch(dtype, vec, inter, [&](auto t, auto v, auto g, const Divisor& by) {
     using E = ElemOf<decltype(t)>;
     swiglu_pack8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const E*>(h), h_stride, num_rows, inter, static_cast<E*>(act), static_cast<uint8_t*>(codes),
+        static_cast<const E*>(h), h_stride, num_rows, inter, by, static_cast<E*>(act), static_cast<uint8_t*>(codes),
         static_cast<uint8_t*>(exponents));
   });
 }
@@ -577,11 +605,11 @@ int kf_swiglu_backward8(const void* codes, const void* exponents, const void* gr
     return KF_ERR_INVALID_ARGUMENT;
   const bool vec = vec_rows(grad_act, grad_stride, inter, dtype) && vec_rows(grad_h, inter, inter, dtype) &&
                    (!act || vec_rows(act, inter, inter, dtype)) && aligned(codes, 8);
-  return launch(dtype, vec, inter, [&](auto t, auto v, auto g) {
+  return launch(dtype, vec, inter, [&](auto t, auto v, auto g, const Divisor& by) {
     using E = ElemOf<decltype(t)>;
     swiglu_backward8_kernel<E, decltype(v)::value, decltype(g)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(exponents), static_cast<const E*>(grad_act),
-        grad_stride, num_rows, inter, static_cast<E*>(grad_h), static_cast<E*>(act));
+        grad_stride, num_rows, inter, by, static_cast<E*>(grad_h), static_cast<E*>(act));
   });
 }
 
