@@ -311,10 +311,10 @@ int kf_combine_backward(const void* grad_output, const void* rows, int32_t dtype
  * = code * 2^(exponent - 127) with one exponent per row and 128 columns, the
  * smallest (>= 1) that holds the block's finite values within 448.  Values that
  * are not finite are kept as NaN.  Codes end at 240 where 256 * 2^e is beyond the
- * type.  kf_restore8 writes the values back: row i of output is row i, or, with
- * pair_row (int32 [num_rows, top_k]) and row_pair (int32 [out_rows]) of
- * kf_sort_tokens, token t's row goes to the rows pair_row[t, :], and the rows
- * that row_pair gives no pair are zero.
+ * type.  kf_restore8 writes the values back.  With top_k 0 (no maps) row i of output
+ * is row i.  With top_k > 0 and pair_row (int32 [num_rows, top_k]) and row_pair
+ * (int32 [out_rows]) of kf_sort_tokens, token t's row goes to the rows
+ * pair_row[t, :], and the rows that row_pair gives no pair are zero.
  */
 int kf_pack8(const void* x, int32_t dtype, int64_t x_stride, int32_t num_rows, int32_t width, void* codes,
              void* exponents, void* stream);

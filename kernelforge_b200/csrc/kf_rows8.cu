@@ -553,8 +553,9 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
                 void* stream) {
   if (!valid_rows(num_rows, width, dtype) || !valid_rows(out_rows, width, dtype)) return KF_ERR_INVALID_ARGUMENT;
   if (num_rows > 0 && (!codes || !exponents)) return KF_ERR_INVALID_ARGUMENT;
-  const bool sorted = row_pair != nullptr;
-  if (sorted ? (top_k < 1 || top_k > KF_SORT_MAX_TOP_K || !valid_tokens(num_rows) || (num_rows > 0 && !pair_row))
+  const bool sorted = top_k != 0;
+  if (sorted ? (top_k < 1 || top_k > KF_SORT_MAX_TOP_K || !valid_tokens(num_rows) || (num_rows > 0 && !pair_row) ||
+                (out_rows > 0 && !row_pair))
              : out_rows != num_rows)
     return KF_ERR_INVALID_ARGUMENT;
   if (out_rows == 0) return KF_OK;

@@ -180,6 +180,14 @@ def test_sort_without_tokens_or_rows():
     out, order = train.sort_tokens(x, ids, 12, max_rows=0)
     assert out.shape == (0, 32) and (order.pair_row == -1).all() and int(order.counts[0]) == 6
     assert not train.combine_tokens(out, order, torch.ones(3, 2).cuda()).any()
+    assert train.restore8(train.pack8(x), order).shape == (0, 32)
+    xg, yg, wg = x.clone().requires_grad_(True), out.clone().requires_grad_(True), torch.ones(3, 2).cuda().requires_grad_(True)
+    assert not torch.autograd.grad(train.sort_tokens(xg, ids, 12, max_rows=0)[0], xg, out)[0].any()
+    dy, dw = torch.autograd.grad(train.combine_tokens(yg, order, wg), (yg, wg), x)
+    assert dy.shape == (0, 32) and not dw.any()
+    none = train.sort_tokens(x[:0], ids[:0], 12, row_align=4, max_rows=8)[1]
+    assert not train.restore8(train.pack8(x[:0]), none).any() and not train.combine_tokens_backward(
+        x[:0], torch.ones(8, 32).cuda(), none, torch.ones(0, 2).cuda())[0].any()
     assert train.combine_tokens(torch.empty(0, 32).cuda(), train.TokenOrder(
         torch.empty(0, 2, dtype=torch.int32).cuda(), torch.empty(0, dtype=torch.int32).cuda(), order.counts, order.starts)).shape == (0, 32)
     assert train.pack8(torch.empty(0, 32).cuda()).codes.shape == (0, 32)

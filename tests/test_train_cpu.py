@@ -158,7 +158,7 @@ def test_the_8_bit_entry_points_refuse_bad_arguments_before_device_work():
     for i, v in ((0, NULL), (0, vp(33)), (1, 3), (2, -1), (3, -1), (4, 0), (4, (1 << 20) + 1), (5, NULL), (6, NULL)):
         assert lib.kf_pack8(*(v if j == i else a for j, a in enumerate(ok))) == 1
     ok = (SOME, SOME, 0, 4, 64, SOME, SOME, 2, 8, SOME, NULL)
-    for i, v in ((0, NULL), (1, NULL), (2, 9), (3, -1), (3, (1 << 24) + 1), (4, 0), (5, NULL), (7, 0), (7, 17), (8, -1), (9, NULL)):
+    for i, v in ((0, NULL), (1, NULL), (2, 9), (3, -1), (3, (1 << 24) + 1), (4, 0), (5, NULL), (6, NULL), (7, 0), (7, -1), (7, 17), (8, -1), (9, NULL)):
         assert lib.kf_restore8(*(v if j == i else a for j, a in enumerate(ok))) == 1
     assert lib.kf_restore8(SOME, SOME, 0, 4, 64, NULL, NULL, 0, 5, SOME, NULL) == 1   # without an order the rows stay as many
     ok = (SOME, 0, 128, 4, 64, SOME, SOME, SOME, NULL)
