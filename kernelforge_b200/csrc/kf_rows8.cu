@@ -282,8 +282,8 @@ __device__ __forceinline__ Unit unit_of(int slices, const Divisor& by) {
 // most an eighth of the warps half empty, else one.
 inline bool pairs_of_slices(int slices) { return slices % 2 == 0 || slices >= 7; }
 
-// Bound by issuing its instructions as much as by memory: 19 us = 4.6 TB/s for 4096 rows
-// of 7168 bf16 columns, 12.7 us = 5.8 TB/s for 2048 of fp32.
+// Bound by issuing its instructions as much as by memory: 19 us = 4.7 TB/s for 4096 rows
+// of 7168 bf16 columns, 11.3 us = 6.5 TB/s for 2048 of fp32.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t stride, int R, int W,
                                                          const Divisor by, uint8_t* __restrict__ codes,
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
 }
 
 // h = [up | gate]: act = up * silu(gate), and h kept in 8 bits (each half's blocks begin at its own column 0).
-// 97 us = 5.5 TB/s for 32768 rows of 2048 bf16 columns each (bound by issue and memory alike: 140 us with divisions
+// 94 us = 5.7 TB/s for 32768 rows of 2048 bf16 columns each (bound by issue and memory alike: 140 us with divisions
 // and a check per element); fp32 rows 6.8 TB/s.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restrict__ h, int64_t stride, int R, int I,
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
 }
 
 // From the kept values u, g and d = dL/dact: du = d g s, dg = d u (s + g s (1 - s)), act = u g s, with s = sigmoid(g).
-// One pass: 102 us = 6.6 TB/s for 32768 rows of 2048 bf16 columns, bound by memory (133 us before its sigmoid took 4
+// One pass: 104 us = 6.4 TB/s for 32768 rows of 2048 bf16 columns, bound by memory (133 us before its sigmoid took 4
 // instructions).
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
