@@ -2,5 +2,6 @@
 
 ``kernelforge_b200.kernel`` is a drop-in for the reference operator
 ``solution/triton/kernel.py::kernel``; the compute runs in ``libkf_moe.so``.
+``kernelforge_b200.train`` has the operators of training around a caller's own expert products.
 """
 from .binding import experts, kernel, route  # noqa: F401

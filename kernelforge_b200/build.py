@@ -106,7 +106,7 @@ def _runtime_cxx_flags() -> list:
         for line in f:
             path = line.rstrip("\n").split(None, 5)[-1]
             if os.path.basename(path).startswith("libstdc++.so"):
-                return ["-nostdlib++", path]
+                return [path]   # ahead of the compiler's own -lstdc++, which then adds nothing
     return []
 
 

@@ -158,6 +158,23 @@ def test_rows_in_place_of_other_layouts(h, dtype):
     R.close(dy, R.combine_grads(torch.ones(t, h), wide[:, 2:2 + h].cpu(), ref[0], ref[1], w)[0], dtype, 0.0)
 
 
+def test_gradients_of_broadcast_inputs():
+    """One row for every token and one weight row for all: torch sums what the operators return."""
+    g = torch.Generator().manual_seed(4)
+    t, k, h = 30, 4, 72
+    ids = _ids(t, k, g)
+    row = torch.randn(1, h, generator=g).cuda().requires_grad_(True)
+    rows, order = train.sort_tokens(row.expand(t, h), ids.cuda(), 256)
+    grad = torch.randn(t * k, h, generator=g)
+    d, = torch.autograd.grad(rows, row, grad.cuda())
+    R.close(d, grad.double().sum(0, keepdim=True), torch.float32, t * k * U * grad.double().abs().sum(0, keepdim=True))
+    w = torch.rand(1, k, generator=g).cuda().requires_grad_(True)
+    dout = torch.randn(t, h, generator=g)
+    dw, = torch.autograd.grad(train.combine_tokens(rows.detach(), order, w.expand(t, k)), w, dout.cuda())
+    _, want, mag = R.combine_grads(dout, rows.detach().cpu(), order.pair_row.cpu(), order.row_pair.cpu(), w.detach().cpu().expand(t, k))
+    R.close(dw, want.sum(0, keepdim=True), torch.float32, (_dot_slack(h) + t * U) * mag.sum(0, keepdim=True))
+
+
 def test_sort_of_repeated_and_foreign_ids():
     ids = torch.tensor([[3, 3, 3], [300, -5, 3], [2 ** 31 - 1, -2 ** 31, 255], [0, 255, 0]], dtype=torch.int32)
     x = torch.randn(4, 16)
@@ -242,6 +259,19 @@ def test_route_gradient_at_the_ends():
     # sigmoids down to e^-100 lose their last bits as fp32 subnormals: what they weigh is below 1e-30
     R.close(dl, want, torch.float32, 2.0 ** -19 * mag + 1e-30)
     assert not dl[3].any()
+
+
+def test_route_gradient_of_repeated_ids():
+    """A repeated id (outside the routing's contract) gets the sum of its choices' gradients."""
+    g = torch.Generator().manual_seed(2)
+    logits = torch.randn(9, 256, generator=g)
+    ids = torch.stack([torch.randperm(256, generator=g)[:8] for _ in range(9)]).to(torch.int32)
+    ids[1, 3] = ids[1, 6]
+    ids[2] = 255
+    ids[5, :4] = ids[5, 4:]
+    gw = torch.randn(9, 8, generator=g)
+    want, mag = R.route_grad(logits, ids, gw, 2.5)
+    R.close(train.route_backward(logits.cuda(), ids.cuda(), gw.cuda(), 2.5), want, torch.float32, 2.0 ** -19 * mag)
 
 
 # --------------------------------------------------------------------- 8 bits --
