@@ -11,6 +11,8 @@ sigmoid passes on at most whole.  Where e^-g leaves fp32's normal numbers
 (g below -87.3, 1 + e^-g above 2^126) the sigmoid, at most 2^-126, may come out as zero: FAR of
 the magnitudes around it.
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -596,6 +598,68 @@ def test_on_a_device_that_is_not_current():
     want = _training_calls(*i)
     got = _training_calls(*(v.to("cuda:1") for v in i))
     assert all(o.device.index == 1 and torch.equal(o.cpu(), w.cpu()) for o, w in zip(got, want))
+
+
+class _Guarded:
+    """Output buffers inside larger ones whose other bytes must stay as they are."""
+
+    def __init__(self):
+        self.all = []
+
+    def __call__(self, nbytes, offset=0):
+        big = torch.full((nbytes + 1024 + offset,), 0xA5, dtype=torch.uint8, device="cuda")
+        self.all.append((big, 512 + offset, nbytes))
+        return ctypes.c_void_p(big.data_ptr() + 512 + offset)
+
+    def check(self):
+        for big, at, n in self.all:
+            assert (big[:at] == 0xA5).all() and (big[at + n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("t,k,h,align,rows", [(1, 1, 1, 1, 1), (5, 3, 257, 8, 40), (40, 8, 1031, 1, 320), (3, 16, 8, 128, 1024),
+                                              (33, 2, 264, 16, 32), (2000, 8, 24, 8, 17600), (130, 5, 130, 1, 0)])
+def test_nothing_outside_the_outputs_is_written(t, k, h, align, rows, dtype):
+    """The C entry points on buffers between guards, also of elements off 16-byte boundaries."""
+    lib, null, es = B.library(), ctypes.c_void_p(0), 4 if dtype == 2 else 2
+    vp, i32, i64, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
+    lib.kf_sort_tokens.argtypes = [vp, i32, i64, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.kf_sort_workspace_bytes.restype = sz
+    lib.kf_combine_tokens.argtypes = [vp, i32, i64, i32, vp, vp, i32, i32, i32, vp, vp]
+    lib.kf_combine_backward.argtypes = [vp, vp, i32, i64, i32, vp, vp, vp, i32, i32, i32, vp, vp, vp]
+    lib.kf_pack8.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp]
+    lib.kf_restore8.argtypes = [vp, vp, i32, i32, i32, vp, vp, i32, i32, vp, vp]
+    lib.kf_swiglu_pack8.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp]
+    lib.kf_swiglu_backward8.argtypes = [vp, vp, vp, i32, i64, i32, i32, vp, vp, vp]
+    torch.cuda.synchronize()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for offset in (0, es, 8 * es):
+        new = _Guarded()
+        src = torch.zeros(2 * t * h + 64, dtype=torch.float32, device="cuda")
+        x = vp(src.data_ptr() + offset)
+        ids = torch.randint(0, 256, (t, k), device="cuda", dtype=torch.int32)
+        w = torch.ones(t, k, device="cuda")
+        pr, rp, counts, starts, out = new(4 * t * k), new(4 * rows), new(1024), new(1028), new(rows * h * es, offset)
+        need = lib.kf_sort_workspace_bytes(t, k, 256)
+        assert lib.kf_sort_tokens(x, dtype, h, vp(ids.data_ptr()), t, k, h, 256, 0, align, rows, out, pr, rp, counts, starts,
+                                  new(need), need, stream) == 0
+        y, dr, dw = new(t * h * es, offset), new(rows * h * es, offset), new(4 * t * k)
+        wp = vp(w.data_ptr())
+        assert lib.kf_combine_tokens(out, dtype, h, rows, pr, wp, t, k, h, y, stream) == 0
+        assert lib.kf_combine_backward(x, out, dtype, h, rows, pr, rp, wp, t, k, h, dr, dw, stream) == 0
+        assert lib.kf_combine_backward(x, null, dtype, h, rows, pr, rp, wp, t, k, h, dr, null, stream) == 0
+        assert lib.kf_combine_backward(x, out, dtype, h, rows, pr, rp, wp, t, k, h, null, dw, stream) == 0
+        nb = (h + 127) // 128
+        codes, exps = new(t * h, offset // es), new(t * nb)
+        assert lib.kf_pack8(x, dtype, h, t, h, codes, exps, stream) == 0
+        assert lib.kf_restore8(codes, exps, dtype, t, h, null, null, 0, t, new(t * h * es, offset), stream) == 0
+        assert lib.kf_restore8(codes, exps, dtype, t, h, pr, rp, k, rows, out, stream) == 0
+        act, codes, exps = new(t * h * es, offset), new(2 * t * h, offset // es), new(2 * t * nb)
+        assert lib.kf_swiglu_pack8(x, dtype, 2 * h, t, h, act, codes, exps, stream) == 0
+        assert lib.kf_swiglu_pack8(x, dtype, 2 * h, t, h, act, null, null, stream) == 0
+        assert lib.kf_swiglu_backward8(codes, exps, x, dtype, h, t, h, new(2 * t * h * es, offset), act, stream) == 0
+        torch.cuda.synchronize()
+        new.check()
 
 
 def test_rows_past_32_bit_offsets():
