@@ -12,6 +12,8 @@
 //
 // (The layer's input format, quantize_rows_kernel, has fp32 scales absmax / 448 as
 // the reference fixes them, solution/triton/kernel.py:126-141, and no way back.)
+#include <type_traits>
+
 #include <cuda_fp8.h>
 
 #include "kf_elem.cuh"
@@ -435,9 +437,36 @@ __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restr
   }
 }
 
+// The fp32 bits of the largest magnitude of a lane's elements; NaN counts as the largest.
+__device__ __forceinline__ uint32_t largest(const Raw8<float>& r) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, r.x[i] & 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ uint32_t largest(const Raw8<__nv_bfloat16>& r) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, r.x[i] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16) << 16;
+}
+
+// From u, g, s = sigmoid(g) and d = dL/dact: act, and the gradients in place of u and g.  dg = d u f with
+// f = s + g s (1 - s), at most 1.1.  kFar: d u alone may be beyond fp32; f then goes into the larger of the two, so
+// that nothing on the way is beyond fp32 or below its normal numbers unless the product is.  (With f always in one of
+// them, u f would vanish for a small u and f, and exceed fp32 for a large u, where d makes up for it.)
+template <bool kFar>
+__device__ __forceinline__ void gate(float s, float d, float& u, float& g, float& act) {
+  const float gs = g * s, f = fmaf(gs, 1.0f - s, s), t = d * u;
+  act = u * gs;
+  g = t * f;
+  if (kFar && fabsf(t) == __uint_as_float(0x7f800000u)) g = fabsf(u) >= fabsf(d) ? u * f * d : d * f * u;
+  u = d * gs;
+}
+
 // From the kept values u, g and d = dL/dact: du = d g s, dg = d u (s + g s (1 - s)), act = u g s, with s = sigmoid(g).
-// One pass: 104 us = 6.4 TB/s for 32768 rows of 2048 bf16 columns, bound by memory (133 us before its sigmoid took 4
-// instructions).
+// One pass: 108 us = 6.2 TB/s for 32768 rows of 2048 bf16 columns, bound by memory and issue (133 us before its sigmoid
+// took 4 instructions).  Telling the lanes whose d u may be beyond fp32 takes 4 us of it, a check per element 10.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ exps,
@@ -463,6 +492,17 @@ __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_
     load_scales<T, kVec>(er, n, lane, su[i]);
     load_scales<T, kVec>(er + nb, n, lane, sg[i]);
   }
+  bool far = false;   // whether some d u of this lane may be beyond fp32 (a NaN among d says so too); of fp16 none is
+  if constexpr (!std::is_same_v<T, __half>) {
+    uint32_t top = 0u;
+    float scale = 0.f;
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      top = max(top, largest(rd[i]));
+      scale = fmaxf(scale, fmaxf(su[i][0], su[i][1]));
+    }
+    far = !(__uint_as_float(top) * (448.f * scale) < __uint_as_float(0x7f800000u));
+  }
 #pragma unroll
   for (int i = 0; i < kGroup; ++i) {
     const int c = (unit.slice + i) * kSlice, n = I - c;
@@ -471,14 +511,12 @@ __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_
     to_floats(rd[i], d);
     decode8(qu[i], su[i], u);
     decode8(qg[i], sg[i], g);
+    if (!far) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float s = sigmoid<T>(g[j]);
-      const float gs = g[j] * s;
-      a[j] = u[j] * gs;
-      const float dg = d[j] * u[j] * fmaf(gs, 1.0f - s, s);
-      u[j] = d[j] * gs;
-      g[j] = dg;
+      for (int j = 0; j < 8; ++j) gate<false>(sigmoid<T>(g[j]), d[j], u[j], g[j], a[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gate<true>(sigmoid<T>(g[j]), d[j], u[j], g[j], a[j]);
     }
     store_raw8<T, kVec>(dh + r * 2 * I + c, n, lane, from_floats<T>(u));
     store_raw8<T, kVec>(dh + r * 2 * I + I + c, n, lane, from_floats<T>(g));

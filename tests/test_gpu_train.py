@@ -371,6 +371,39 @@ def test_swiglu_of_far_gates(dtype):
     assert torch.isfinite(dh).all() and torch.isfinite(again).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_swiglu_gradient_of_large_values(dtype):
+    """A gate gradient d u (s + g s (1 - s)) whose product d u alone is beyond fp32, and one whose product u (s + ..) is."""
+    big = 60000.0 if dtype == torch.float16 else 1e20
+    pairs = [(big, big), (-big, big), (big, -big)]
+    pairs += [] if dtype == torch.float16 else [(3e38, 0.1), (0.1, 3e38), (3e38, 3e38), (3e38, -2.0), (1e30, 1e9)]
+    gates = [-1000.0, -90, -86, -60, -50, -30, -10, -1, -1e-3, 0, 1e-3, 1, 2.4, 10, 1000]
+    # one value a block: each is kept on its own scale
+    u, d, gate = (torch.tensor(v) for v in zip(*[(a, b, g) for a, b in pairs for g in gates]))
+    u, d, gate = u[:, None].to(dtype), d[:, None].to(dtype), gate[:, None].to(dtype)
+    _, kept = train.swiglu_pack8(torch.cat([u, gate], 1).cuda())
+    ku, kg, dd = R.to_8_bits(u)[0], R.to_8_bits(gate)[0], d.double()
+    dh, act = train.swiglu_backward8(kept, d.cuda())
+    du, dg, a, mag = R.swiglu_grads(ku, kg, dd)
+    near = _sigmoid_slack(kg, dtype)
+    R.close(act, a, dtype, near * a.abs() + FAR * (ku * kg).abs())
+    R.close(dh[:, :1], du, dtype, near * du.abs() + FAR * (dd * kg).abs())
+    R.close(dh[:, 1:], dg, dtype, near * mag + FAR * (dd * ku).abs() * (1 + kg.abs()))
+    # a gradient that is no number hides no neighbour's product
+    row = torch.full((1, 8), 1.0).to(dtype)
+    row[0, 3] = float("nan")
+    d = torch.full((1, 8), big).to(dtype)
+    d[0, 5] = float("nan")
+    _, kept = train.swiglu_pack8(torch.cat([row * big, torch.full((1, 8), -50.0).to(dtype)], 1).cuda())
+    dg = train.swiglu_backward8(kept, d.cuda())[0][:, 8:].cpu()
+    assert torch.equal(torch.isnan(dg[0]), torch.tensor([i in (3, 5) for i in range(8)]))
+    fine = torch.tensor([0, 1, 2, 4, 6, 7])
+    ku, dd = R.to_8_bits(row * big)[0][:, fine], d[:, fine].double()
+    kg = R.to_8_bits(torch.full((1, 8), -50.0).to(dtype))[0][:, fine]
+    _, want, _, mag = R.swiglu_grads(ku, kg, dd)
+    R.close(dg[:, fine], want, dtype, _sigmoid_slack(kg, dtype) * mag)
+
+
 # ------------------------------------------------------------------- together --
 
 
