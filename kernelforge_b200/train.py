@@ -32,6 +32,8 @@ import torch
 
 from . import binding as B
 
+BLOCK = 128   # columns of a row that share an exponent in 8 bits
+
 
 class TokenOrder(NamedTuple):
     """Where ``sort_tokens`` put each (token, choice) pair; all int32 on the tokens' device.
@@ -46,10 +48,32 @@ class TokenOrder(NamedTuple):
 
 
 class Rows8(NamedTuple):
-    """Rows in 8 bits: ``codes * 2 ** (exponents - 127)``, one exponent per row and 128 columns."""
+    """Rows in 8 bits: ``codes * 2 ** (exponents - 127)``, one exponent per row and 128 columns.
+
+    ``pack8`` counts the columns from the row's first, ``swiglu_pack8`` from the first of each half; the shapes
+    alone do not tell the two apart, so each returns a type of its own, and an operator that reads the other
+    layout refuses it (unless a half is a multiple of 128 wide, where both are the same).  A ``Rows8`` that a
+    caller puts together from its parts is read as the operator reads rows.
+    """
     codes: torch.Tensor      # e4m3 [R, W]
     exponents: torch.Tensor  # uint8 [R, ceil(W / 128)] (for SwiGLU's input 2 ceil(I / 128): up's, then gate's)
     dtype: torch.dtype       # of the rows they were made from
+
+
+class WholeRows8(Rows8):
+    """What ``pack8`` returns: blocks begin at the row's first column."""
+    __slots__ = ()
+
+
+class HalvesRows8(Rows8):
+    """What ``swiglu_pack8`` returns: blocks begin at the first column of each half."""
+    __slots__ = ()
+
+
+def _refuse_layout(kept: Rows8, other: type, what: str) -> None:
+    if isinstance(kept, other) and kept.codes.shape[-1] % (2 * BLOCK):
+        raise RuntimeError(f"{what} reads rows whose blocks of {BLOCK} columns begin elsewhere than those of this "
+                           f"{type(kept).__name__} of {kept.codes.shape[-1]} columns")
 
 
 def route(routing_logits: torch.Tensor, routing_bias: torch.Tensor, routed_scaling_factor):
@@ -115,11 +139,12 @@ def pack8(x: torch.Tensor) -> Rows8:
     No gradient passes.
     """
     codes, exponents = B.extension().pack8(x)
-    return Rows8(codes, exponents, x.dtype)
+    return WholeRows8(codes, exponents, x.dtype)
 
 
 def restore8(kept: Rows8, order: Optional[TokenOrder] = None) -> torch.Tensor:
-    """The rows that ``kept`` stands for, or with ``order`` its tokens' rows in expert order (zeros elsewhere)."""
+    """The rows that ``kept`` (of ``pack8``) stands for, or with ``order`` its tokens' rows in expert order (zeros elsewhere)."""
+    _refuse_layout(kept, HalvesRows8, "restore8")
     return B.extension().restore8(kept.codes, kept.exponents, kept.dtype, order.pair_row if order is not None else None,
                                   order.row_pair if order is not None else None)
 
@@ -132,9 +157,10 @@ def swiglu(h: torch.Tensor) -> torch.Tensor:
 def swiglu_pack8(h: torch.Tensor):
     """``(act [R, I], Rows8)``: SwiGLU and its input in 8 bits, in one pass.  No gradient passes."""
     act, codes, exponents = B.extension().swiglu_pack8(h)
-    return act, Rows8(codes, exponents, h.dtype)
+    return act, HalvesRows8(codes, exponents, h.dtype)
 
 
 def swiglu_backward8(kept: Rows8, grad_act: torch.Tensor, need_act: bool = True):
     """``(grad_h [R, 2 I], act [R, I] or None)`` from SwiGLU's kept input, in the type of ``grad_act``."""
+    _refuse_layout(kept, WholeRows8, "swiglu_backward8")
     return tuple(B.extension().swiglu_backward8(kept.codes, kept.exponents, grad_act, need_act))

@@ -404,6 +404,28 @@ def test_swiglu_gradient_of_large_values(dtype):
     R.close(dg[:, fine], want, dtype, _sigmoid_slack(kg, dtype) * mag)
 
 
+@pytest.mark.parametrize("n", [70, 96, 100, 127, 128, 256])
+def test_rows_in_8_bits_know_where_their_blocks_begin(n):
+    """SwiGLU's blocks begin at each half's first column: rows kept one way are not read the other way unless both agree."""
+    g = torch.Generator().manual_seed(n)
+    h = torch.randn(6, 2 * n, generator=g)
+    h[:, n:] *= 1000                                  # a half's scale would not fit the other's values
+    d = torch.randn(6, n, generator=g).cuda()
+    whole, (_, halves) = train.pack8(h.cuda()), train.swiglu_pack8(h.cuda())
+    want = train.swiglu_backward8(halves, d)[0]
+    again = train.Rows8(halves.codes, halves.exponents, halves.dtype)      # as a caller's autograd function puts it together
+    assert torch.equal(train.swiglu_backward8(again, d)[0], want)
+    assert isinstance(whole, train.Rows8) and isinstance(halves, train.Rows8) and len(halves) == 3
+    if n % 128:
+        with pytest.raises(RuntimeError, match="restore8"):
+            train.restore8(halves)
+        with pytest.raises(RuntimeError, match="swiglu_backward8"):
+            train.swiglu_backward8(whole, d)
+    else:
+        assert torch.equal(train.restore8(halves).cpu().double(), R.to_8_bits(h)[0])
+        assert torch.equal(train.swiglu_backward8(whole, d)[0], want)
+
+
 # ------------------------------------------------------------------- together --
 
 

@@ -188,6 +188,24 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+@pytest.mark.parametrize("n", [1, 64, 100, 128, 129, 384])
+def test_rows_in_8_bits_kept_the_other_way_are_refused(n):
+    """SwiGLU's blocks begin at each half's first column; where that is elsewhere, the other way's rows are refused."""
+    codes = torch.zeros(3, 2 * n, dtype=torch.float8_e4m3fn)
+    whole = train.WholeRows8(codes, torch.zeros(3, -(-2 * n // 128), dtype=torch.uint8), torch.float32)
+    halves = train.HalvesRows8(codes, torch.zeros(3, 2 * -(-n // 128), dtype=torch.uint8), torch.float32)
+    message = "no CPU fallback" if n % 128 == 0 else "begin elsewhere"
+    for kept in (halves, halves._replace(dtype=torch.bfloat16)):
+        with pytest.raises(RuntimeError, match=message):
+            train.restore8(kept)
+    with pytest.raises(RuntimeError, match=message):
+        train.swiglu_backward8(whole, torch.zeros(3, n))
+    for call in (lambda: train.restore8(whole), lambda: train.swiglu_backward8(halves, torch.zeros(3, n)),
+                 lambda: train.restore8(train.Rows8(*halves)), lambda: train.swiglu_backward8(train.Rows8(*whole), torch.zeros(3, n))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
 def test_every_operator_is_documented():
     for name in ("route", "route_backward", "sort_tokens", "sort_tokens_backward", "combine_tokens",
                  "combine_tokens_backward", "pack8", "restore8", "swiglu", "swiglu_pack8", "swiglu_backward8"):
