@@ -88,6 +88,17 @@ void refuse_shared_leaf(const Tensor& t) {
               "or capture a detached copy that requires grad");
 }
 
+// The operators have no forward-mode rule.  A tensor that carries a tangent need not require a gradient, so without
+// this check it would take the way past the autograd function, and its tangent would be lost without an error.  (The
+// tangent is undefined where forward mode is switched off.)
+void refuse_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what,
+              " has no forward-mode derivative: an argument carries a tangent (torch.autograd.forward_ad)");
+}
+void refuse_tangent(const std::optional<Tensor>& t, const char* what) {
+  if (t.has_value()) refuse_tangent(*t, what);
+}
+
 void refuse_double_backward(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is not twice differentiable (backward with create_graph=True)");
 }
@@ -180,6 +191,7 @@ struct SortFn : public torch::autograd::Function<SortFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_double_backward("sort_tokens");
+    refuse_tangent(grads[0], "sort_tokens");
     Tensor dx;
     if (grads[0].defined())
       dx = combine_forward(expect_rows(grads[0], "grad of rows"), ctx->get_saved_variables()[0], Tensor());
@@ -190,6 +202,7 @@ struct SortFn : public torch::autograd::Function<SortFn> {
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> sort_tokens(const Tensor& x_in, const Tensor& topk_idx,
                                                                int64_t num_experts, int64_t expert_offset,
                                                                int64_t row_align, std::optional<int64_t> max_rows) {
+  refuse_tangent(x_in, "sort_tokens");
   refuse_shared_leaf(x_in);
   const Tensor x = expect_rows(x_in, "x");
   const int64_t T = x.size(0);
@@ -218,6 +231,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> sort_tokens(const Tensor& x_i
 }
 
 Tensor sort_tokens_backward(const Tensor& grad_rows, const Tensor& pair_row, const Tensor& row_pair) {
+  refuse_tangent(grad_rows, "sort_tokens_backward");
   const Tensor g = expect_rows(grad_rows, "grad_rows");
   const Order o = expect_order(pair_row, row_pair, g.device());
   TORCH_CHECK(g.size(0) == o.row_pair.size(0), "grad_rows has ", g.size(0), " rows, the order ", o.row_pair.size(0));
@@ -235,6 +249,7 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_double_backward("combine_tokens");
+    refuse_tangent(grads[0], "combine_tokens");
     Tensor dr, dw;
     if (grads[0].defined()) {
       const auto saved = ctx->get_saved_variables();
@@ -254,6 +269,8 @@ Tensor expect_weight(const std::optional<Tensor>& w, const Order& o, const at::D
 
 Tensor combine_tokens(const Tensor& rows_in, const Tensor& pair_row, const Tensor& row_pair,
                       const std::optional<Tensor>& topk_weight) {
+  refuse_tangent(rows_in, "combine_tokens");
+  refuse_tangent(topk_weight, "combine_tokens");
   refuse_shared_leaf(rows_in);
   if (topk_weight.has_value()) refuse_shared_leaf(*topk_weight);
   const Tensor rows = expect_rows(rows_in, "rows");
@@ -268,6 +285,7 @@ Tensor combine_tokens(const Tensor& rows_in, const Tensor& pair_row, const Tenso
 std::tuple<Tensor, Tensor> combine_tokens_backward(const Tensor& grad_output, const Tensor& rows_in,
                                                    const Tensor& pair_row, const Tensor& row_pair,
                                                    const Tensor& topk_weight) {
+  for (const Tensor* t : {&grad_output, &rows_in, &topk_weight}) refuse_tangent(*t, "combine_tokens_backward");
   const Tensor g = expect_rows(grad_output, "grad_output");
   const at::Device dev = g.device();
   const Order o = expect_order(pair_row, row_pair, dev);
@@ -283,6 +301,8 @@ std::tuple<Tensor, Tensor> combine_tokens_backward(const Tensor& grad_output, co
 
 Tensor route_backward(const Tensor& routing_logits, const Tensor& topk_idx, const Tensor& grad_weight,
                       double routed_scaling_factor) {
+  refuse_tangent(routing_logits, "route_backward");
+  refuse_tangent(grad_weight, "route_backward");
   check_cuda(routing_logits, "routing_logits");
   const at::Device dev = routing_logits.device();
   TORCH_CHECK(routing_logits.dim() == 2, "routing_logits must be [T, 256]");
@@ -333,6 +353,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 };
 
 std::tuple<Tensor, Tensor> route(const Tensor& routing_logits, const Tensor& routing_bias, double rsf) {
+  refuse_tangent(routing_logits, "route");
   refuse_shared_leaf(routing_logits);
   check_cuda(routing_logits, "routing_logits");
   const at::Device dev = routing_logits.device();
@@ -420,6 +441,7 @@ std::tuple<Tensor, Tensor, Tensor> swiglu_pack8(const Tensor& h) { return swiglu
 
 std::tuple<Tensor, Tensor> swiglu_backward8(const Tensor& codes_in, const Tensor& exps_in, const Tensor& grad_act,
                                             bool need_act) {
+  refuse_tangent(grad_act, "swiglu_backward8");
   auto [codes, exps] = expect_kept(codes_in, exps_in, 2);
   const Tensor g = expect_rows(grad_act, "grad_act");
   const int64_t R = codes.size(0), I = codes.size(1) / 2;
@@ -450,6 +472,7 @@ struct SwigluFn : public torch::autograd::Function<SwigluFn> {
 };
 
 Tensor swiglu(const Tensor& h) {
+  refuse_tangent(h, "swiglu");
   refuse_shared_leaf(h);
   if (wants_grad(h)) return SwigluFn::apply(h);
   return std::get<0>(swiglu_forward(h, false));

@@ -19,7 +19,9 @@ scratch from torch's caching allocator and never synchronises, so it can be capt
 a CUDA graph, after one call outside a capture (the library's set-up on a device).  A
 captured call on a leaf tensor that an eager autograd graph still holds raises.  Errors raise
 ``RuntimeError``.  Sums are fp32 in a fixed order: equal inputs give equal bits.  The gradients
-are not differentiable again: a backward pass with ``create_graph=True`` raises.
+are not differentiable again: a backward pass with ``create_graph=True`` raises.  There are no
+forward-mode derivatives: a tensor that carries a tangent (``torch.autograd.forward_ad``) raises, but
+in ``pack8`` and ``swiglu_pack8``, which pass no derivative at all.
 
 The reference has no training path; its routing, sort and combine are inside ``kernel``
 (``solution/triton/kernel.py:1842-1925``).

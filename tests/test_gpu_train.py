@@ -15,6 +15,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from kernelforge_b200 import binding as B
 from kernelforge_b200 import train
@@ -465,6 +466,38 @@ def test_no_second_derivative():
     for out in (rows, train.swiglu(x), train.combine_tokens(rows, order)):
         with pytest.raises(RuntimeError, match="not twice differentiable"):
             torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """No operator has a forward-mode rule: a tangent raises, in the forward and in the backward pass, instead of getting lost."""
+    g = torch.Generator().manual_seed(21)
+    x, ids = torch.randn(4, 32, generator=g).cuda(), torch.tensor([[0, 1]] * 4, dtype=torch.int32).cuda()
+    logits, bias = torch.randn(4, 256, generator=g).cuda(), torch.zeros(256, dtype=torch.bfloat16).cuda()
+    w = torch.ones(4, 2).cuda()
+    rows, order = train.sort_tokens(x, ids, 8)
+    act, kept = train.swiglu_pack8(x)
+    leaves = [a.clone().requires_grad_(True) for a in (x, rows, w, logits)]
+    outs = [(train.sort_tokens(leaves[0], ids, 8)[0], leaves[0]), (train.swiglu(leaves[0]), leaves[0]),
+            (train.combine_tokens(leaves[1], order, w), leaves[1]), (train.combine_tokens(rows, order, leaves[2]), leaves[2]),
+            (train.route(leaves[3], bias, 2.5)[1], leaves[3])]
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t.detach(), torch.ones_like(t))
+
+        calls = [lambda: train.route(dual(logits), bias, 2.5), lambda: train.sort_tokens(dual(x), ids, 8),
+                 lambda: train.combine_tokens(dual(rows), order, w), lambda: train.combine_tokens(rows, order, dual(w)),
+                 lambda: train.combine_tokens(dual(rows), order), lambda: train.swiglu(dual(x)),
+                 lambda: train.sort_tokens_backward(dual(rows), order), lambda: train.combine_tokens_backward(dual(x), rows, order, w),
+                 lambda: train.combine_tokens_backward(x, rows, order, dual(w)), lambda: train.swiglu_backward8(kept, dual(act)),
+                 lambda: train.route_backward(logits, ids.repeat(1, 4), dual(w.repeat(1, 4)), 2.5)]
+        calls += [lambda out=out, leaf=leaf: torch.autograd.grad(out, leaf, dual(out)) for out, leaf in outs]
+        for i, call in enumerate(calls):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was accepted")
+        assert torch.equal(train.swiglu(x), act)      # without a tangent, inside the level too
+    for out, leaf in outs:                            # and the reverse mode as ever
+        assert torch.isfinite(torch.autograd.grad(out, leaf, torch.ones_like(out))[0]).all()
 
 
 def _layer(x, logits, bias, w13, w2, products):

@@ -5,6 +5,7 @@ import inspect
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from kernelforge_b200 import binding as B
 from kernelforge_b200 import train
@@ -204,6 +205,27 @@ def test_rows_in_8_bits_kept_the_other_way_are_refused(n):
                  lambda: train.restore8(train.Rows8(*halves)), lambda: train.swiglu_backward8(train.Rows8(*whole), torch.zeros(3, n))):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
+
+
+def test_tangents_are_refused_before_any_other_check():
+    """No operator has a forward-mode rule, so none takes a tensor with a tangent and loses it."""
+    x, ids = torch.zeros(2, 16), torch.zeros(2, 1, dtype=torch.int32)
+    w, bias, logits = torch.zeros(2, 1), torch.zeros(256, dtype=torch.bfloat16), torch.zeros(2, 256)
+    order = train.TokenOrder(ids, torch.zeros(2, dtype=torch.int32), ids, ids)
+    kept = train.Rows8(torch.zeros(2, 32, dtype=torch.float8_e4m3fn), torch.zeros(2, 2, dtype=torch.uint8), torch.float32)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: train.route(dual(logits), bias, 1.0), lambda: train.route_backward(dual(logits), ids, x, 1.0),
+                 lambda: train.route_backward(logits, ids, dual(x), 1.0), lambda: train.sort_tokens(dual(x), ids, 4),
+                 lambda: train.sort_tokens_backward(dual(x), order), lambda: train.combine_tokens(dual(x), order),
+                 lambda: train.combine_tokens(x, order, dual(w)), lambda: train.combine_tokens_backward(dual(x), x, order, w),
+                 lambda: train.combine_tokens_backward(x, dual(x), order, w), lambda: train.combine_tokens_backward(x, x, order, dual(w)),
+                 lambda: train.swiglu(dual(x)), lambda: train.swiglu_backward8(kept, dual(x))]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
 
 
 def test_every_operator_is_documented():
