@@ -73,19 +73,31 @@ Tensor new_tensor(at::IntArrayRef shape, at::ScalarType dtype, const at::Device&
 
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
-// During a stream capture a leaf whose gradient accumulator already lives on another
-// stream -- an eager graph of the same leaf is still alive -- is refused: the backward
-// pass would make that stream wait for the capturing one, which invalidates the capture
-// inside the autograd engine.  `t`: an argument as the caller gave it.
+// During a stream capture a leaf whose gradient accumulator lives on the default stream
+// -- an eager graph of the same leaf, made there, is still alive -- is refused: the
+// backward pass makes that stream wait for the capturing one, which the legacy stream
+// cannot, and invalidates the capture inside the autograd engine.  Any other stream joins
+// the capture by waiting (a warm-up on a side stream whose graph is still alive), unless
+// another capture holds it.  `t`: an argument as the caller gave it.
 void refuse_shared_leaf(const Tensor& t) {
   if (!t.defined() || !t.is_cuda() || !t.is_leaf() || !wants_grad(t)) return;
-  const at::cuda::CUDAStream now = at::cuda::getCurrentCUDAStream(t.device().index());
+  const c10::DeviceIndex dev = t.device().index();
+  const at::cuda::CUDAStream now = at::cuda::getCurrentCUDAStream(dev);
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(now.stream(), &cap) != cudaSuccess || cap == cudaStreamCaptureStatusNone) return;
+  unsigned long long capture = 0, other = 0;
+  if (cudaStreamGetCaptureInfo(now.stream(), &cap, &capture) != cudaSuccess || cap == cudaStreamCaptureStatusNone) return;
   const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
-  TORCH_CHECK(!acc || !acc->stream().has_value() || *acc->stream() == now.unwrap(),
-              "a captured call on a leaf tensor whose eager autograd graph is still alive: release that graph first, "
-              "or capture a detached copy that requires grad");
+  if (!acc || !acc->stream().has_value() || *acc->stream() == now.unwrap()) return;
+  const at::cuda::CUDAStream its(*acc->stream());
+  bool joins = its != at::cuda::getDefaultCUDAStream(dev);
+  if (joins) {
+    cap = cudaStreamCaptureStatusNone;
+    joins = cudaStreamGetCaptureInfo(its.stream(), &cap, &other) == cudaSuccess &&
+            (cap == cudaStreamCaptureStatusNone || (cap == cudaStreamCaptureStatusActive && other == capture));
+  }
+  TORCH_CHECK(joins,
+              "a captured call on a leaf tensor whose eager autograd graph is still alive on the default stream (or in "
+              "another capture): release that graph first, or capture a detached copy that requires grad");
 }
 
 // The operators have no forward-mode rule.  A tensor that carries a tangent need not require a gradient, so without

@@ -17,7 +17,9 @@ order; ``swiglu_backward8`` returns the activation along with the gradient.
 Every call runs on the current stream of its tensors' device, allocates its outputs and
 scratch from torch's caching allocator and never synchronises, so it can be captured into
 a CUDA graph, after one call outside a capture (the library's set-up on a device).  A
-captured call on a leaf tensor that an eager autograd graph still holds raises.  Errors raise
+captured call on a leaf tensor that an eager autograd graph of the default stream still holds
+raises, as its backward pass could not be captured (a graph made on a side stream does no harm;
+arguments computed from such a leaf, a cast or a view of it, are not looked through).  Errors raise
 ``RuntimeError``.  Sums are fp32 in a fixed order: equal inputs give equal bits.  The gradients
 are not differentiable again: a backward pass with ``create_graph=True`` raises.  There are no
 forward-mode derivatives: a tensor that carries a tangent (``torch.autograd.forward_ad``) raises, but

@@ -657,6 +657,46 @@ def test_capture_with_an_eager_graph_of_the_same_leaf_is_refused():
     assert (dx == 1).all() and also.requires_grad and fourth[1].requires_grad
 
 
+@pytest.mark.parametrize("backward", [True, False], ids=["backward", "grad"])
+def test_capture_with_a_graph_of_the_same_leaf_on_a_side_stream(backward):
+    """Warm-up on a side stream whose graph still lives, then a capture: that stream joins the capture."""
+    g = torch.Generator().manual_seed(31)
+    x, w, logits = (torch.randn(8, n, generator=g).cuda().requires_grad_(True) for n in (64, 1, 256))
+    bias, ids = torch.zeros(256, dtype=torch.bfloat16).cuda(), torch.zeros(8, 1, dtype=torch.int32).cuda()
+    douts = [torch.randn(8, n, generator=g).cuda() for n in (64, 8, 32)]
+    leaves = (x, w, logits)
+
+    def step():
+        rows, order = train.sort_tokens(x, ids, 4)
+        return train.combine_tokens(rows, order, w), train.route(logits, bias, 2.5)[1], train.swiglu(x)
+
+    def gradients(outs):
+        if not backward:
+            return torch.autograd.grad(outs, leaves, douts, retain_graph=True)
+        for leaf in leaves:
+            leaf.grad = None
+        torch.autograd.backward(outs, douts, retain_graph=True)
+        return [leaf.grad for leaf in leaves]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = step()                                # lives through the capture
+        want = [a.clone() for a in gradients(alive)]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for leaf in leaves:
+        leaf.grad = None
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = gradients(step())
+    for a in got:
+        a.detach().zero_()
+    gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(alive) == 3
+
+
 def test_two_streams_at_once():
     """Calls in flight on two streams share nothing."""
     inputs = [_inputs(3, 6000), _inputs(4, 6000)]
