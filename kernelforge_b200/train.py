@@ -15,7 +15,8 @@ A product written as its own autograd function can keep its operands in 8 bits a
 order; ``swiglu_backward8`` returns the activation along with the gradient.
 
 Every call runs on the current stream of its tensors' device, allocates its outputs and
-scratch from torch's caching allocator and never synchronises, so it can be captured into
+scratch from torch's caching allocator and never synchronises (but to read a
+``routed_scaling_factor`` that is a CUDA tensor; pass a number), so it can be captured into
 a CUDA graph, after one call outside a capture (the library's set-up on a device).  A
 captured call on a leaf tensor that an eager autograd graph of the default stream still holds
 raises, as its backward pass could not be captured (a graph made on a side stream does no harm;
@@ -80,12 +81,19 @@ def _refuse_layout(kept: Rows8, other: type, what: str) -> None:
                            f"{type(kept).__name__} of {kept.codes.shape[-1]} columns")
 
 
+def _factor(v) -> float:
+    if isinstance(v, torch.Tensor) and v.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a routed_scaling_factor that is a CUDA tensor has to be read back, which a stream capture "
+                           "does not allow: pass a number")
+    return B._scalar_float(v)
+
+
 def route(routing_logits: torch.Tensor, routing_bias: torch.Tensor, routed_scaling_factor):
     """As ``binding.route``, with weights that are differentiable in the logits.
 
     The choice of experts has no gradient, and the bias takes part in the choice only.
     """
-    return B.extension().route(routing_logits, routing_bias, B._scalar_float(routed_scaling_factor))
+    return B.extension().route(routing_logits, routing_bias, _factor(routed_scaling_factor))
 
 
 def route_backward(routing_logits: torch.Tensor, topk_idx: torch.Tensor, grad_weight: torch.Tensor,
@@ -94,7 +102,7 @@ def route_backward(routing_logits: torch.Tensor, topk_idx: torch.Tensor, grad_we
 
     Ids outside [0, 256) count as no choice.
     """
-    return B.extension().route_backward(routing_logits, topk_idx, grad_weight, B._scalar_float(routed_scaling_factor))
+    return B.extension().route_backward(routing_logits, topk_idx, grad_weight, _factor(routed_scaling_factor))
 
 
 def sort_tokens(x: torch.Tensor, topk_idx: torch.Tensor, num_experts: int, expert_offset: int = 0, *,

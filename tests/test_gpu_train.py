@@ -697,6 +697,27 @@ def test_capture_with_a_graph_of_the_same_leaf_on_a_side_stream(backward):
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(alive) == 3
 
 
+def test_a_factor_on_the_gpu_is_refused_in_a_capture():
+    """Reading it back would end the capture; the refusal leaves the capture whole.  Outside it is read."""
+    logits, bias = torch.randn(8, 256).cuda(), torch.zeros(256, dtype=torch.bfloat16).cuda()
+    factor = torch.tensor(2.5).cuda()
+    ids, w = train.route(logits, bias, 2.5)
+    assert torch.equal(train.route(logits, bias, factor)[1], w)
+    want = train.route_backward(logits, ids, w, 2.5)
+    assert torch.equal(train.route_backward(logits, ids, w, factor), want)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        for call in (lambda: train.route(logits, bias, factor), lambda: train.route_backward(logits, ids, w, factor)):
+            with pytest.raises(RuntimeError, match="pass a number"):
+                call()
+        again = train.route(logits, bias, torch.tensor(2.5))[1]      # on the host it may be a tensor
+        grad = train.route_backward(logits, ids, w, 2.5)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, w) and torch.equal(grad, want)
+
+
 def test_two_streams_at_once():
     """Calls in flight on two streams share nothing."""
     inputs = [_inputs(3, 6000), _inputs(4, 6000)]
