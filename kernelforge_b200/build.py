@@ -21,10 +21,16 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libkf_moe.so")
 EXT = os.path.join(PKG, "_kf_torch.so")
-EXT_SOURCES = ["kf_torch_ext.cpp", "kf_torch_train.cpp"]
-SOURCES = ["kf_route_permute.cu", "kf_grouped_gemm.cu", "kf_moe_api.cu",
-           "kf_moe_noalloc.cu", "kf_ep.cu", "kf_quant.cu", "kf_sort.cu", "kf_rows8.cu", "kf_route_grad.cu"]
-HEADERS = ["kf_ptx.cuh", "kf_internal.cuh", "kf_quant.cuh", "kf_fp8.cuh", "kf_elem.cuh"]
+# The layer and, beside it, the training operators: a copy of the package without train.py (the packed solution, whose
+# entry point calls none of them) builds the layer alone, in 11 s of nvcc instead of 29.
+LAYER_EXT_SOURCES = ["kf_torch_ext.cpp"]
+LAYER_SOURCES = ["kf_route_permute.cu", "kf_grouped_gemm.cu", "kf_moe_api.cu",
+                 "kf_moe_noalloc.cu", "kf_ep.cu", "kf_quant.cu"]
+LAYER_HEADERS = ["kf_ptx.cuh", "kf_internal.cuh", "kf_quant.cuh", "kf_fp8.cuh"]
+HAS_TRAIN = os.path.exists(os.path.join(PKG, "train.py"))
+EXT_SOURCES = LAYER_EXT_SOURCES + (["kf_torch_train.cpp"] if HAS_TRAIN else [])
+SOURCES = LAYER_SOURCES + (["kf_sort.cu", "kf_rows8.cu", "kf_route_grad.cu"] if HAS_TRAIN else [])
+HEADERS = LAYER_HEADERS + (["kf_elem.cuh"] if HAS_TRAIN else [])
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v", f"-I{INCLUDE}"]
@@ -111,7 +117,8 @@ def _runtime_cxx_flags() -> list:
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> str:
-    """The torch extension (``kf_torch_ext.cpp``, ``kf_torch_train.cpp``), linked against ``libkf_moe.so``."""
+    """The torch extension (``kf_torch_ext.cpp`` and, with the training operators, ``kf_torch_train.cpp``), linked
+    against ``libkf_moe.so``."""
     if not force and ext_up_to_date():
         return EXT
     import ctypes
@@ -122,7 +129,8 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     bdir = os.path.join(PKG, "_build", "torch_ext")
     os.makedirs(bdir, exist_ok=True)
     cpp_extension.load(name="_kf_torch", sources=[os.path.join(CSRC, f) for f in EXT_SOURCES], extra_include_paths=[INCLUDE],
-                       extra_cflags=["-O3"], extra_ldflags=[f"-L{PKG}", "-lkf_moe", *_runtime_cxx_flags()], build_directory=bdir,
+                       extra_cflags=["-O3"] + ([] if HAS_TRAIN else ["-DKF_NO_TRAIN"]),
+                       extra_ldflags=[f"-L{PKG}", "-lkf_moe", *_runtime_cxx_flags()], build_directory=bdir,
                        with_cuda=True, verbose=verbose)
     tmp = EXT + ".tmp"
     shutil.copyfile(os.path.join(bdir, "_kf_torch.so"), tmp)

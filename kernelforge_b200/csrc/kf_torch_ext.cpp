@@ -29,7 +29,9 @@
 
 #include "kf_moe.h"
 
+#ifndef KF_NO_TRAIN   // defined by a build without the training operators
 void register_train(pybind11::module_& m);  // kf_torch_train.cpp
+#endif
 
 namespace {
 
@@ -171,5 +173,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kernel", &kernel, "the fused MoE layer (kf_moe_forward); returns bf16 [T, 7168]");
   m.def("read_status", &read_status, "synchronise and return, then clear, the device status of this module's calls");
   m.def("release_workspaces", &release_workspaces, "drop the cached workspaces");
+#ifndef KF_NO_TRAIN
   register_train(m);
+#endif
 }

@@ -15,8 +15,8 @@ its output), and the entry point ``kernelforge_b200/binding.py::kernel`` whose
 ten positional parameters are the reference's.
 
 The sources are exactly what the entry point needs: the Python binding and its
-build step, the CUDA sources, the PyTorch C++ extension over the C ABI and the
-C-ABI header.  On first call the binding compiles ``libkf_moe.so`` for sm_100a
+build step, the CUDA sources of the layer, the PyTorch C++ extension over the C ABI and
+the C-ABI header (the training operators, which the entry point does not call, stay out).  On first call the binding compiles ``libkf_moe.so`` for sm_100a
 and the extension ``_kf_torch.so`` from them (``build.py``); it has no CPU
 fallback.  How the contest harness's own CUDA builder treats these
 sources is not known here (the harness is not available), so the JSON is
@@ -43,7 +43,8 @@ def source_files() -> List[str]:
     """Repository-relative paths of every file the packed solution carries."""
     from . import build
     files = [os.path.join("kernelforge_b200", f) for f in PY_SOURCES]
-    files += [os.path.join("kernelforge_b200", "csrc", f) for f in build.SOURCES + build.HEADERS + build.EXT_SOURCES]
+    files += [os.path.join("kernelforge_b200", "csrc", f) for f in build.LAYER_SOURCES + build.LAYER_HEADERS +
+              build.LAYER_EXT_SOURCES]
     files.append(os.path.join("include", "kf_moe.h"))
     return files
 

@@ -48,6 +48,24 @@ def test_unpack_rejects_escaping_paths(tmp_path):
         P.unpack({"sources": [{"path": "../evil.py", "content": "x"}]}, str(tmp_path))
 
 
+def test_packed_sources_are_what_the_entry_point_needs(tmp_path):
+    """No source of the training operators, which nothing in the package could call, and none missing from the build."""
+    from kernelforge_b200 import build
+    sol = P.solution_dict()
+    names = {os.path.basename(s["path"]) for s in sol["sources"]}
+    assert names == {*P.PY_SOURCES, *build.LAYER_SOURCES, *build.LAYER_HEADERS, *build.LAYER_EXT_SOURCES, "kf_moe.h"}
+    assert not names & {"train.py", "kf_sort.cu", "kf_rows8.cu", "kf_route_grad.cu", "kf_elem.cuh", "kf_torch_train.cpp"}
+    for s in sol["sources"]:
+        if s["path"].endswith((".cu", ".cuh", ".cpp")):
+            own = [line.split('"')[1] for line in s["content"].splitlines() if line.startswith('#include "')]
+            assert set(own) <= names, s["path"]
+    P.unpack(sol, str(tmp_path))
+    code = ("import sys, os; sys.path.insert(0, '.'); from kernelforge_b200 import build as b; print(b.HAS_TRAIN, "
+            "all(os.path.exists(os.path.join(b.CSRC, f)) for f in b.SOURCES + b.HEADERS + b.EXT_SOURCES))")
+    r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["False", "True"], r.stderr[-2000:]
+
+
 @pytest.mark.skipif(not os.path.exists(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")), reason="needs nvcc")
 def test_unpacked_sources_build_and_import(tmp_path):
     """The sources alone rebuild libkf_moe.so for sm_100a and its torch extension, and the entry point
