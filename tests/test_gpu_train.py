@@ -330,6 +330,24 @@ def test_rows_in_8_bits_in_expert_order(case, dtype):
     assert torch.equal(back.cpu(), R.gather(R.to_8_bits(x)[0].to(dtype), ref[1], case["k"]))
 
 
+MANY_CHOICES = [
+    # more than eight choices: two batches of rows per slice, in the 16-byte and in the plain forms
+    dict(t=37, k=9, h=264, experts=256, offset=0, align=8, masked=0.2),
+    dict(t=3000, k=16, h=72, experts=64, offset=32, align=1, masked=0.0),
+    dict(t=20, k=12, h=7168, experts=256, offset=0, align=16, masked=0.0),
+    dict(t=21, k=13, h=1031, experts=200, offset=0, align=1, masked=0.3),
+    dict(t=90, k=16, h=520, experts=256, offset=0, align=1, masked=0.0, max_rows=900),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", MANY_CHOICES, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_more_than_eight_choices(case, dtype):
+    test_sort_and_its_gradient(case, dtype)
+    test_combine_and_its_gradients(case, dtype)
+    test_rows_in_8_bits_in_expert_order(case, dtype)
+
+
 # --------------------------------------------------------------------- swiglu --
 
 
