@@ -348,6 +348,48 @@ def test_more_than_eight_choices(case, dtype):
     test_rows_in_8_bits_in_expert_order(case, dtype)
 
 
+MANY_STEPS = [
+    # more tokens than blocks that stay, and several steps per warp and token: the load stream is a step ahead of the sum
+    dict(t=400, k=3, h=7168, experts=256, offset=0, align=1, masked=0.2),
+    dict(t=400, k=8, h=7168, experts=128, offset=64, align=8, masked=0.2),
+    dict(t=400, k=2, h=7168, experts=256, offset=0, align=1, masked=0.2),
+    dict(t=400, k=11, h=7168, experts=256, offset=0, align=1, masked=0.2),
+    dict(t=600, k=8, h=2056, experts=256, offset=0, align=1, masked=0.2),
+    dict(t=500, k=4, h=3848, experts=256, offset=0, align=1, masked=0.2),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", MANY_STEPS, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_several_tokens_a_block_and_steps_a_warp(case, dtype):
+    """Random weights and rows of their own per pair: a step summed with another token's or choice's weight or row fails."""
+    test_combine_and_its_gradients(case, dtype)
+
+
+def test_combine_past_32_bit_offsets_tells_weights_and_rows_apart():
+    """More than 2^31 elements of rows, each row and weight its own, against sums in 64 bits at some of the tokens."""
+    t, h, k = 40960, 7168, 8
+    g = torch.Generator(device="cuda").manual_seed(10)
+    ids = torch.randn(t, 256, generator=g, device="cuda").topk(k, dim=1).indices.to(torch.int32)
+    _, order = train.sort_tokens(torch.zeros(t, 1, dtype=torch.bfloat16, device="cuda"), ids, 256)
+    rows = torch.randn(t * k, h, generator=g, device="cuda", dtype=torch.bfloat16)
+    assert rows.numel() > 2 ** 31 and int(order.pair_row.max()) == t * k - 1
+    w = torch.rand(t, k, generator=g, device="cuda") + 0.1
+    dout = torch.randn(t, h, generator=g, device="cuda", dtype=torch.bfloat16)
+    out = train.combine_tokens(rows, order, w)
+    drows, dw = train.combine_tokens_backward(dout, rows, order, w)
+    last = order.row_pair[-200:].long() // k          # the tokens of the last rows
+    pick = torch.cat([torch.arange(50, device="cuda"), torch.randint(0, t, (250,), device="cuda", generator=g), last])
+    at = order.pair_row[pick].long()
+    picked = rows[at.reshape(-1)].double().reshape(pick.numel(), k, h)
+    terms = picked * w[pick, :, None].double()
+    R.close(out[pick], terms.sum(1).cpu(), torch.bfloat16, (k + 1) * U * terms.abs().sum(1).cpu())
+    prod = picked * dout[pick, None].double()
+    R.close(dw[pick], prod.sum(2).cpu(), torch.float32, _dot_slack(h) * prod.abs().sum(2).cpu())
+    want = (dout[pick, None].double() * w[pick, :, None].double()).reshape(-1, h).cpu()
+    R.close(drows[at.reshape(-1)], want, torch.bfloat16, U * want.abs())
+
+
 # --------------------------------------------------------------------- swiglu --
 
 
