@@ -279,8 +279,8 @@ int kf_moe_route_backward(const float* routing_logits, const int32_t* topk_idx, 
  * num_rows is a multiple of row_align.  A pair whose row would lie at or past
  * num_rows is dropped (its pair_row is -1; counts still counts it): pass at least
  * T * K + min(T * K, E) * (row_align - 1) to keep all.  `workspace`:
- * kf_sort_workspace_bytes(T, K, E) bytes (none for small calls).  Ids repeated in a token's choices are
- * separate pairs.
+ * kf_sort_workspace_bytes(T, K, E) bytes (none for small calls), 4-byte aligned.  Ids repeated in a token's
+ * choices are separate pairs.
  */
 size_t kf_sort_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t num_experts);
 int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t* topk_idx, int32_t num_tokens,

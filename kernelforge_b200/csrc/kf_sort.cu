@@ -935,7 +935,7 @@ int kf_sort_tokens(const void* x, int32_t dtype, int64_t x_stride, const int32_t
     return KF_ERR_INVALID_ARGUMENT;
   if (!elem_aligned(x, dtype) || !elem_aligned(rows, dtype)) return KF_ERR_INVALID_ARGUMENT;
   const size_t need = kf_sort_workspace_bytes(num_tokens, top_k, num_experts);
-  if (need && !workspace) return KF_ERR_INVALID_ARGUMENT;
+  if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3u))) return KF_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < need) return KF_ERR_WORKSPACE_TOO_SMALL;
   int sms = 0;
   const int rc = device_ready(&sms);

@@ -128,6 +128,11 @@ def test_sort_refuses_a_small_workspace_and_sizes_it():
     assert _sort(T=65536, K=8, R=65536 * 8, wsb=16) == 2
 
 
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_sort_refuses_a_workspace_off_its_alignment(offset):
+    assert _sort(T=65536, K=8, R=65536 * 8, ws=vp(256 + offset)) == 1
+
+
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(K=0), dict(K=17), dict(H=0), dict(dtype=5), dict(R=-1), dict(pr=NULL),
                                  dict(out=NULL), dict(out=vp(257)), dict(rows=NULL), dict(rows=vp(1)), dict(stride=-3)])
 def test_combine_refuses_bad_arguments_before_device_work(bad):
