@@ -243,7 +243,9 @@ int kf_quantize_hidden(const void* x, int32_t num_tokens, void* out, float* out_
  * Operators around a user's own expert products (the reference has none of
  * them: its sort, SwiGLU and combine live inside kernel() without gradients).
  * Rows are bf16, fp16 or fp32 (`dtype`), of any width; 16-byte aligned rows whose
- * width is a multiple of 8 take 16-byte accesses, others one element at a time.
+ * width is a multiple of 8 take 16-byte accesses, others 4-byte ones (and one element
+ * at a time at a row's end; their 8-bit codes a byte at a time), at about half the speed
+ * for 16-bit types.
  * A *_stride is the number of elements between an input's consecutive rows;
  * outputs are dense.  Sums are fp32, in a fixed order, rounded once.
  */
@@ -327,6 +329,7 @@ int kf_restore8(const void* codes, const void* exponents, int32_t dtype, int32_t
  * [R, I], with h kept in 8 bits: codes [R, 2 I], exponents [R, 2 ceil(I / 128)], the
  * blocks of each half beginning at its own first column (both NULL: act alone).  The backward pass reads
  * what was kept: grad_h [R, 2 I], and act as the kept values give it (act may be NULL).
+ * A sigmoid below 2^-126 (a gate under -87) may count as zero.
  */
 int kf_swiglu_pack8(const void* h, int32_t dtype, int64_t h_stride, int32_t num_rows, int32_t inter, void* act,
                     void* codes, void* exponents, void* stream);

@@ -284,8 +284,10 @@ __device__ __forceinline__ Unit unit_of(int slices, const Divisor& by) {
 // most an eighth of the warps half empty, else one.
 inline bool pairs_of_slices(int slices) { return slices % 2 == 0 || slices >= 7; }
 
-// Bound by issuing its instructions as much as by memory: 19 us = 4.7 TB/s for 4096 rows
-// of 7168 bf16 columns, 11.3 us = 6.5 TB/s for 2048 of fp32.
+// 60 us = 5.8 TB/s for 16384 rows of 7168 bf16 columns, 43 us = 6.8 TB/s for 8192 of fp32; 16.5 us = 5.3 TB/s for 4096
+// of bf16 among others and 19 us alone: memory and issue share it (of the issue slots 73 % while blocks run, 56 % over
+// the launch), and such a launch's first and last blocks.  Off 16 bytes codes go a byte at a time: 28 us for 4096
+// rows of 7167 bf16 columns, 27 us of fp32.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t stride, int R, int W,
                                                          const Divisor by, uint8_t* __restrict__ codes,
@@ -323,7 +325,8 @@ __device__ __forceinline__ Raw8<T> restored(uint2 codes, const float (&s)[2]) {
   return from_floats<T>(v);
 }
 
-// Rows as they were.  12.8 us = 6.9 TB/s for 4096 rows of 7168 bf16 columns.
+// Rows as they were.  54 us = 6.6 TB/s for 16384 rows of 7168 bf16 columns, 46 us = 6.3 TB/s for 8192 of fp32; off 16
+// bytes 28 us for 4096 rows of 7167 bf16 columns, 32 us of fp32.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __restrict__ codes,
                                                             const uint8_t* __restrict__ exps, int R, int W,
@@ -350,8 +353,8 @@ __global__ void __launch_bounds__(kThreads) restore8_kernel(const uint8_t* __res
 // Rows in expert order: a block holds a token's row across its warps, two slices
 // each, decodes it once and stores it K times (as scatter_rows_kernel, whose reason
 // for one block per token holds here too).  The first blocks zero the rows of no pair.
-// 93 us = 5.9 TB/s for 4096 tokens of 7168 bf16 columns into 36608 rows; a warp per
-// output row, which decodes a row K times, took 214 us.
+// 93 us = 6.0 TB/s for 4096 tokens of 7168 bf16 columns into 36608 rows (fp32 175 us = 6.2 TB/s, 7167 bf16 columns
+// 117 us); a warp per output row, which decodes a row K times, took 214 us.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int T_, int W,
@@ -393,8 +396,9 @@ __global__ void __launch_bounds__(kScatterWarps * 32) restore8_sorted_kernel(
 }
 
 // h = [up | gate]: act = up * silu(gate), and h kept in 8 bits (each half's blocks begin at its own column 0).
-// 94 us = 5.7 TB/s for 32768 rows of 2048 bf16 columns each (bound by issue and memory alike: 140 us with divisions
-// and a check per element); fp32 rows 6.8 TB/s.
+// 90 us = 6.0 TB/s for 32768 rows of 2048 bf16 columns each (bound by issue and memory alike: 140 us with divisions
+// and a check per element), 139 us = 6.8 TB/s of fp32; the activation alone 62 us = 6.5 TB/s.  Rows of 2047 bf16
+// columns, whose codes go a byte at a time, 188 us.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_pack8_kernel(const T* __restrict__ h, int64_t stride, int R, int I,
                                                                 const Divisor by, T* __restrict__ act,
@@ -465,8 +469,9 @@ __device__ __forceinline__ void gate(float s, float d, float& u, float& g, float
 }
 
 // From the kept values u, g and d = dL/dact: du = d g s, dg = d u (s + g s (1 - s)), act = u g s, with s = sigmoid(g).
-// One pass: 108 us = 6.2 TB/s for 32768 rows of 2048 bf16 columns, bound by memory and issue (133 us before its sigmoid
-// took 4 instructions).  Telling the lanes whose d u may be beyond fp32 takes 4 us of it, a check per element 10.
+// One pass: 99 us = 6.8 TB/s for 32768 rows of 2048 bf16 columns, without act 84 us = 6.4 TB/s, bound by memory (the
+// sigmoid in 15 instructions took 30 us more).  Telling the lanes whose d u may be beyond fp32 takes 5 us of the 84
+// and none of the 99, a check per element 10.  fp32: 180 us = 6.7 TB/s.  2047 bf16 columns: 227 us.
 template <typename T, bool kVec, int kGroup>
 __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ exps,

@@ -8,9 +8,11 @@
 //   backward  drows[r] = w[p] dout[t], dw[t,k] = <dout[t], rows[pair_row[t,k]]>
 //
 // A sort is one launch when it is small, else placing (after a histogram, for many
-// pairs) and the scatter, chained by programmatic launches.  All of it but the order
-// (some 9 us at 32768 pairs, of them 3 us histogram) is bound by memory: every row is
-// read or written once, at 5.6 to 6.6 TB/s where a plain copy reaches 6.55.
+// pairs) and the scatter, chained by programmatic launches.  In the 16-byte forms all
+// but the order (some 9 us at 32768 pairs, of them 3 us histogram) is bound by memory:
+// every row is read or written once, in large calls at 5.5 to 6.8 TB/s where a plain
+// copy reaches 6.55.  Rows off 16 bytes run at 2.3 to 4.9 TB/s in 16-bit types (the
+// narrow ones slowest) and 5.5 to 6.6 in fp32.
 //
 // The reference sorts and combines inside its kernel() only, for its own FP8
 // layer and without gradients (solution/triton/kernel.py:46-82, :1920-1925).
@@ -511,11 +513,12 @@ struct CombineArgs {
   int T, K, H, R;
 };
 
-// Forward.  A block of up to 14 warps (7 for fp32) stays and loops over tokens, as many
-// blocks as fit the SMs; each warp sums one step while the next one's rows arrive, and
-// the pairs of the token after that are on their way.  Measured (K = 8, bf16; 4096
-// tokens of 7168 columns and 16384 of 2048): 81 and 91 us = 6.5 and 6.6 TB/s, against
-// 94 and 106 us with the rows loaded to registers.
+// Forward.  A block of up to 14 warps (7 for fp32) stays and loops over tokens, on each
+// SM as many blocks as make about that many warps of eight rows (one block at 7168
+// columns); each warp sums one step while the next one's rows arrive, and the pairs of
+// the token after that are on their way.  Measured (K = 8, bf16; 4096 tokens of 7168
+// columns and 16384 of 2048): 81 and 90 us = 6.5 and 6.7 TB/s, against 94 and 106 us with
+// the rows loaded to registers; fp32, 4096 tokens of 7168 columns: 155 us = 6.8 TB/s.
 constexpr int kForwardStages = 2;
 template <typename T>
 constexpr int kForwardWarps = sizeof(T) == 4 ? 7 : 14;
@@ -607,9 +610,9 @@ __global__ void __launch_bounds__(kForwardWarps<T> * 32) combine_pipe_kernel(con
 // address order (as in scatter_rows_kernel).  The blocks of an SM overlap each other;
 // a warp with several steps issues the next before it sums one.  The first blocks
 // zero the rows without a pair.  Measured (K = 8, bf16; 4096 tokens of 7168 columns,
-// 16384 of 2048): 162 and 180 us = 6.2 and 6.3 TB/s, against 171 and 205 us for
-// blocks that stay and 202 and 239 us with the rows loaded to registers; 14 warps and
-// one stage: 174 and 193 us.
+// 16384 of 2048): 162 to 169 and 180 us = 6.2 to 6.5 and 6.4 TB/s, against 171 and 205
+// us for blocks that stay and 202 and 239 us with the rows loaded to registers; 14 warps
+// and one stage: 174 and 193 us.  fp32, 4096 tokens of 7168 columns: 329 us = 6.4 TB/s.
 constexpr int kBackwardStages = 2;
 constexpr int kBackwardWarps = 7;
 
@@ -777,8 +780,9 @@ template <typename T>
 constexpr int kBatch = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight together
 
 // One warp per (token, slice of 256 columns), consecutive warps on consecutive slices.
-// 25 us = 3.1 TB/s for 4096 tokens of 1031 columns, K = 8, bf16 (rows between two words:
-// bound by the shuffles), 21 us for 1030 columns.
+// 33 us = 2.3 TB/s for 4096 tokens of 1031 columns, K = 8, bf16 (rows between two words:
+// bound by the shuffles; 25 us from the L2), 23 us for 1030 columns; 7167 columns 172 us
+// = 3.1 TB/s; fp32 rows of 7164 columns 161 us = 6.6 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const CombineArgs a) {
   const T* rows = static_cast<const T*>(a.rows);
@@ -810,8 +814,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(const CombineAr
 }
 
 // `warps` warps per token share its slices, `tokens` tokens per block.  The first
-// blocks zero the rows without a pair.  64 us = 2.4 TB/s at the sizes above, 45 us for
-// 1030 columns; with one element per access it took 165 us.
+// blocks zero the rows without a pair.  61 us = 2.5 TB/s for 1031 columns, 43 us for
+// 1030 columns, 295 us = 3.6 TB/s for 7167, fp32 352 us = 6.0 TB/s for 7164; with one
+// element per access 1031 columns took 165 us.
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(const CombineArgs a, int warps, int tokens,
                                                                           unsigned zero_blocks) {

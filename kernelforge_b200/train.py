@@ -162,7 +162,12 @@ def restore8(kept: Rows8, order: Optional[TokenOrder] = None) -> torch.Tensor:
 
 
 def swiglu(h: torch.Tensor) -> torch.Tensor:
-    """``up * silu(gate)`` of ``h`` ``[R, 2 I]`` = [up | gate]; the backward pass reads ``h`` from 8 bits."""
+    """``up * silu(gate)`` of ``h`` ``[R, 2 I]`` = [up | gate]; the backward pass reads ``h`` from 8 bits.
+
+    So its gradient is that of the kept values, in fp32 too: for normally distributed ``h`` it differs from the
+    gradient at ``h`` by 3 % (root mean square; cosine 0.9995).  For that one, take SwiGLU from torch's own
+    operations.  A sigmoid below 2^-126 (a gate under -87) may count as zero.
+    """
     return B.extension().swiglu(h)
 
 
